@@ -16,7 +16,9 @@ FVB_OK = 0
  FVB_ERR_WORKSPACE) = range(1, 6)
 EPI_BF16, EPI_F32_STORE, EPI_F32_ACC, EPI_GEGLU, EPI_QKV_ROPE = range(5)
 ACT_NONE, ACT_GELU_TANH, ACT_SILU = range(3)
-NORM_GEMMA_RMS, NORM_ADA_RMS, NORM_LAYER, NORM_RMS, NORM_ADA_STYLE = range(5)
+(NORM_GEMMA_RMS, NORM_ADA_RMS, NORM_LAYER, NORM_RMS, NORM_ADA_STYLE,
+ NORM_NONE) = range(6)
+NORM_FP8_MAX_DIM = 16384
 
 
 class GemmArgs(C.Structure):
@@ -77,7 +79,46 @@ class ExpertArgs(C.Structure):
                 ('workspace', C.c_void_p), ('workspace_bytes', C.c_int64)]
 
 
+def _args(name, fields):
+    """A ctypes structure from 'p:a i:b l:c f:d d:e' (pointer, int32, int64,
+    float, double)."""
+    kind = {'p': C.c_void_p, 'i': C.c_int32, 'l': C.c_int64, 'f': C.c_float,
+            'd': C.c_double}
+    return type(name, (C.Structure,), {'_fields_': [
+        (f[2:], kind[f[0]]) for f in fields.split()]})
+
+
+NormFp8Args = _args('NormFp8Args', """
+    i:mode i:rows i:dim p:x l:ld_x i:x_f32 p:delta l:ld_delta i:delta_f32
+    p:res l:ld_res p:w p:mod d:eps p:q l:ld_q p:scales l:ld_scales""")
+GemmFp8Args = _args('GemmFp8Args', """
+    p:a l:lda p:a_scale l:ld_as p:b l:ldb p:b_scale l:ld_bs i:m i:n i:k
+    i:epilogue p:out l:ldo""")
+PagedAppendArgs = _args('PagedAppendArgs', """
+    p:q l:q_row_stride l:q_head_stride p:k l:k_row_stride l:k_head_stride
+    p:v l:v_row_stride l:v_head_stride
+    p:q_out l:q_out_row_stride l:q_out_head_stride
+    p:k_cache l:kc_page_stride l:kc_row_stride l:kc_head_stride
+    p:v_cache l:vc_page_stride l:vc_row_stride l:vc_head_stride
+    i:n_pages i:page_size p:slots p:positions p:rope_cs i:max_pos
+    i:rope_interleaved i:tokens i:heads i:kv_heads i:head_dim""")
+PagedAttnArgs = _args('PagedAttnArgs', """
+    p:q l:q_row_stride l:q_head_stride
+    p:k_cache l:kc_page_stride l:kc_row_stride l:kc_head_stride
+    p:v_cache l:vc_page_stride l:vc_row_stride l:vc_head_stride
+    i:n_pages i:page_size p:page_table l:ld_table i:max_pages p:seq_lens
+    p:out l:out_row_stride l:out_head_stride p:lse l:lse_row_stride
+    i:batch i:heads i:kv_heads i:head_dim f:scale
+    p:workspace l:workspace_bytes""")
+
+
 EXPORTS = {
+    'fvb_norm_fp8': (C.c_int, [C.POINTER(NormFp8Args), C.c_void_p]),
+    'fvb_gemm_fp8': (C.c_int, [C.POINTER(GemmFp8Args), C.c_void_p]),
+    'fvb_paged_append': (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),
+    'fvb_paged_attention': (C.c_int, [C.POINTER(PagedAttnArgs), C.c_void_p]),
+    'fvb_paged_attention_workspace_bytes': (C.c_int64,
+                                            [C.POINTER(PagedAttnArgs)]),
     'fvb_expert_step': (C.c_int, [C.POINTER(ExpertArgs), C.c_void_p]),
     'fvb_expert_workspace_bytes': (C.c_int64, [C.POINTER(ExpertArgs)]),
     'fvb_gemm': (C.c_int, [C.POINTER(GemmArgs), C.c_void_p]),

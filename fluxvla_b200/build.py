@@ -2,8 +2,9 @@
 
     python -m fluxvla_b200.build [--verbose]
 
-The library is a single translation unit (csrc/fluxvla_b200.cu including
-the kernel headers) exposing the C ABI of include/fluxvla_b200.h.  It links
+The library is two translation units (csrc/fluxvla_b200.cu and
+csrc/serving_ops.cu with the kernel headers they include), compiled side by
+side, exposing the C ABI of include/fluxvla_b200.h.  It links
 only the CUDA runtime; the driver entry point for tensor-map encoding is
 resolved at run time through cudaGetDriverEntryPoint.
 """
@@ -15,13 +16,14 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SRC = os.path.join(HERE, 'csrc', 'fluxvla_b200.cu')
+SRCS = [os.path.join(HERE, 'csrc', f)
+        for f in ('fluxvla_b200.cu', 'serving_ops.cu')]
 OUT = os.path.join(HERE, 'libfluxvla_b200.so')
 NVCC = os.environ.get('NVCC', '/usr/local/cuda/bin/nvcc')
 
 FLAGS = ['-gencode', 'arch=compute_100a,code=sm_100a', '-lineinfo', '-O3',
-         '-std=c++17', '-Xcompiler', '-fPIC', '-shared',
-         '-I' + os.path.join(ROOT, 'include'), '-lcudart']
+         '-std=c++17', '-Xcompiler', '-fPIC',
+         '-I' + os.path.join(ROOT, 'include')]
 
 
 def sources():
@@ -40,13 +42,24 @@ def needs_build() -> bool:
 def build(verbose: bool = False, force: bool = False) -> str:
     if not force and not needs_build():
         return OUT
-    cmd = [NVCC] + FLAGS + (['-Xptxas', '-v'] if verbose else []) + [
-        SRC, '-o', OUT + '.tmp']
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    objs = [OUT + f'.{i}.o' for i in range(len(SRCS))]
+    flags = FLAGS + (['-Xptxas', '-v'] if verbose else [])
+    jobs = [subprocess.Popen([NVCC] + flags + ['-c', src, '-o', obj],
+                             stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+                             text=True) for src, obj in zip(SRCS, objs)]
+    logs = [j.communicate()[0] for j in jobs]
+    log = ''.join(logs)
+    if any(j.returncode for j in jobs):
+        raise RuntimeError('nvcc failed:\n' + log)
+    r = subprocess.run([NVCC] + FLAGS + ['-shared'] + objs +
+                       ['-lcudart', '-o', OUT + '.tmp'],
+                       capture_output=True, text=True)
+    for obj in objs:
+        os.remove(obj)
     if r.returncode != 0:
         raise RuntimeError('nvcc failed:\n' + r.stdout + r.stderr)
     if verbose:
-        print(r.stdout + r.stderr)
+        print(log)
     os.replace(OUT + '.tmp', OUT)
     return OUT
 

@@ -14,8 +14,9 @@ typedef __nv_bfloat16 bf16;
 
 // Library status word.  Kernels never trap: a wait that runs past its time
 // limit records FVB_ERR_DEVICE_TIMEOUT here and the kernel returns; the host
-// reads it back with fvb_get_device_status().
-__device__ int g_fvb_device_status;
+// reads it back with fvb_get_device_status().  Each translation unit has its
+// own.
+static __device__ int g_fvb_device_status;
 
 // Upper bound for any single spin-wait inside a kernel (nanoseconds).  The
 // longest legitimate wait here is one CTA waiting on a TMA tile or on the MMA

@@ -1,0 +1,351 @@
+// C ABI of the operators that serve several requests at once (declared in
+// include/fluxvla_b200.h): e4m3 norm and product, paged append and attention.
+// Host side: argument checks, tensor maps, launch shapes.  No entry point
+// allocates, synchronises or exits.
+#include "host.cuh"
+
+#include "gemm_fp8.cuh"
+#include "norm_fp8.cuh"
+#include "paged.cuh"
+
+using namespace fvb_host;
+
+// This translation unit's status word (common.cuh), read and reset through
+// fvb_get_device_status.
+int fvb_serving_device_status(int* status, int reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_fvb_device_status, sizeof(int));
+  if (e == cudaSuccess && reset) {
+    const int z = 0;
+    e = cudaMemcpyToSymbol(g_fvb_device_status, &z, sizeof(int));
+  }
+  if (e != cudaSuccess) return fail(FVB_ERR_CUDA, "read status: %s", cudaGetErrorString(e));
+  return FVB_OK;
+}
+
+namespace {
+
+bool aligned(const void* p, int bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+}
+
+// 2-D byte tensor map over [rows, k] (row stride ld bytes), box [box_rows,
+// 128] with the 128-byte swizzle; out-of-range reads fill zeros.
+int make_map_u8(CUtensorMap* m, const void* ptr, int64_t rows, int64_t k, int64_t ld,
+                int box_rows) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) return fail(FVB_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides,
+                   box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(FVB_ERR_INVALID_ARG, "tensor map encode failed (%d)", (int)r);
+  return FVB_OK;
+}
+
+template <typename TX, int DT>
+int launch_norm_fp8(const fvb::n8::Dev& d, int rows, cudaStream_t st) {
+  namespace N = fvb::n8;
+  const int chunks = (d.dim + N::VEC - 1) / N::VEC;
+  if (d.mode == FVB_NORM_NONE) {
+    // no row statistics: runs of 2048 columns, each its own CTA
+    const int t = chunks < 256 ? (chunks + 31) / 32 * 32 : 256;
+    return launch_k("fvb_norm_fp8", N::norm_fp8_kernel<TX, DT, 1>,
+                    dim3(rows, (chunks + t - 1) / t), dim3(t), 0, st, d);
+  }
+  const int vpt = chunks <= N::MAX_THREADS ? 1 : (chunks <= 2 * N::MAX_THREADS ? 2 : 4);
+  const int t = ((chunks + vpt - 1) / vpt + 31) / 32 * 32;
+  if (vpt == 1)
+    return launch_k("fvb_norm_fp8", N::norm_fp8_kernel<TX, DT, 1>, dim3(rows), dim3(t), 0, st, d);
+  if (vpt == 2)
+    return launch_k("fvb_norm_fp8", N::norm_fp8_kernel<TX, DT, 2>, dim3(rows), dim3(t), 0, st, d);
+  return launch_k("fvb_norm_fp8", N::norm_fp8_kernel<TX, DT, 4>, dim3(rows), dim3(t), 0, st, d);
+}
+
+template <typename TX>
+int launch_norm_fp8(const fvb::n8::Dev& d, int delta, int rows, cudaStream_t st) {
+  namespace N = fvb::n8;
+  if (delta == N::DELTA_NONE) return launch_norm_fp8<TX, N::DELTA_NONE>(d, rows, st);
+  if (delta == N::DELTA_F32) return launch_norm_fp8<TX, N::DELTA_F32>(d, rows, st);
+  return launch_norm_fp8<TX, N::DELTA_BF16>(d, rows, st);
+}
+
+template <int BN, bool SWAP, int EPI>
+int launch_gemm_fp8(const CUtensorMap& ma, const CUtensorMap& mb, const fvb::g8::Dev& d,
+                    int tiles, cudaStream_t st) {
+  using C = fvb::g8::Cfg<BN, SWAP>;
+  auto kern = fvb::g8::gemm_fp8_kernel<BN, SWAP, EPI>;
+  if (int r = ensure_smem(reinterpret_cast<const void*>(kern), C::SMEM, "fvb_gemm_fp8")) return r;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * d.cl));
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = d.cl;
+  attrs[0].val.clusterDim.y = 1;
+  attrs[0].val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ma, mb, d);
+  if (e != cudaSuccess)
+    return fail(FVB_ERR_CUDA, "fvb_gemm_fp8: launch failed: %s", cudaGetErrorString(e));
+  return check_launch("fvb_gemm_fp8");
+}
+
+template <int BN, bool SWAP>
+int launch_gemm_fp8(int epi, const CUtensorMap& ma, const CUtensorMap& mb,
+                    const fvb::g8::Dev& d, int tiles, cudaStream_t st) {
+  if (epi == FVB_EPI_BF16) return launch_gemm_fp8<BN, SWAP, FVB_EPI_BF16>(ma, mb, d, tiles, st);
+  if (epi == FVB_EPI_GEGLU) return launch_gemm_fp8<BN, SWAP, FVB_EPI_GEGLU>(ma, mb, d, tiles, st);
+  return launch_gemm_fp8<BN, SWAP, FVB_EPI_F32_STORE>(ma, mb, d, tiles, st);
+}
+
+constexpr int64_t ATTEND_COUNTER_BYTES = 4096;  // one int per CTA
+
+// Launch shape of an attention call: blocks of 8 or 16 heads, one CTA per SM.
+struct AttendShape {
+  int nt, head_blocks, ctas;
+  int64_t off_o, off_ml, bytes;
+};
+
+int attend_prepare(const fvb_paged_attn_args* a, AttendShape* s) {
+  if (!a) return fail(FVB_ERR_INVALID_ARG, "args is NULL");
+  if (a->batch < 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads)
+    return fail(FVB_ERR_INVALID_ARG,
+                "fvb_paged_attention: bad batch %d or heads %d / %d", a->batch, a->heads,
+                a->kv_heads);
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256)
+    return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attention: head_dim %d (64, 128 or 256)",
+                a->head_dim);
+  const int group = a->heads / a->kv_heads;
+  s->nt = group <= 8 ? 1 : 2;
+  s->head_blocks = (group + 8 * s->nt - 1) / (8 * s->nt);
+  s->ctas = sm_count() < 1024 ? sm_count() : 1024;
+  const int64_t rows = 2ll * s->ctas * 8 * s->nt;
+  // the counters keep their place whatever the shape, so that calls of
+  // several shapes may share a workspace one after the other
+  s->off_o = ATTEND_COUNTER_BYTES;
+  s->off_ml = s->off_o + rows * a->head_dim * 4;
+  s->bytes = s->off_ml + rows * 8;
+  return FVB_OK;
+}
+
+template <int D, int NT>
+int launch_attend(const fvb::paged::AttendDev& d, int ctas, cudaStream_t st) {
+  using C = fvb::paged::Cfg<D, NT>;
+  auto kern = fvb::paged::attend_kernel<D, NT>;
+  if (int r = ensure_smem(reinterpret_cast<const void*>(kern), C::SMEM, "fvb_paged_attention"))
+    return r;
+  return launch_k("fvb_paged_attention", kern, dim3(ctas), dim3(fvb::paged::THREADS),
+                  (size_t)C::SMEM, st, d);
+}
+
+}  // namespace
+
+extern "C" {
+
+int fvb_norm_fp8(const fvb_norm_fp8_args* a, void* stream) {
+  if (!a) return fail(FVB_ERR_INVALID_ARG, "args is NULL");
+  if (a->rows < 0 || a->dim <= 0)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_norm_fp8: bad shape %d x %d", a->rows, a->dim);
+  if (a->mode != FVB_NORM_GEMMA_RMS && a->mode != FVB_NORM_ADA_RMS && a->mode != FVB_NORM_RMS &&
+      a->mode != FVB_NORM_NONE)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_norm_fp8: bad mode %d", a->mode);
+  if (a->mode != FVB_NORM_NONE && a->dim > FVB_NORM_FP8_MAX_DIM)
+    return fail(FVB_ERR_UNSUPPORTED, "fvb_norm_fp8: dim %d over %d", a->dim,
+                FVB_NORM_FP8_MAX_DIM);
+  if (!a->x || !a->q || !a->scales)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_norm_fp8: NULL operand");
+  if (a->mode == FVB_NORM_GEMMA_RMS && !a->w)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_norm_fp8: weight required");
+  if (a->mode == FVB_NORM_ADA_RMS && !a->mod)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_norm_fp8: modulation required");
+  if ((a->delta == nullptr) != (a->res == nullptr))
+    return fail(FVB_ERR_INVALID_ARG, "fvb_norm_fp8: delta and res come together");
+  const int groups = (a->dim + 127) / 128;
+  if (a->ld_x < a->dim || a->ld_q < a->dim || a->ld_scales < groups ||
+      (a->delta && (a->ld_delta < a->dim || a->ld_res < a->dim)))
+    return fail(FVB_ERR_INVALID_ARG, "fvb_norm_fp8: a row stride is shorter than its row");
+  if (!(a->eps >= 0)) return fail(FVB_ERR_INVALID_ARG, "fvb_norm_fp8: bad eps");
+  if (a->rows == 0) return FVB_OK;
+  const int xb = a->x_f32 ? 4 : 2, db = a->delta_f32 ? 4 : 2;
+  auto rows16 = [](const void* p, int64_t ld, int eb) { return aligned16(p) && ld * eb % 16 == 0; };
+  fvb::n8::Dev d;
+  d.mode = a->mode;
+  d.x = a->x; d.ld_x = a->ld_x;
+  d.delta = a->delta; d.ld_delta = a->ld_delta;
+  d.res = a->res; d.ld_res = a->ld_res;
+  d.w = (const bf16*)a->w; d.mod = a->mod;
+  d.q = (uint8_t*)a->q; d.ld_q = a->ld_q;
+  d.scales = a->scales; d.ld_scales = a->ld_scales;
+  d.dim = a->dim; d.eps = a->eps;
+  d.vec = rows16(a->x, a->ld_x, xb) && aligned(a->q, 8) && a->ld_q % 8 == 0 &&
+          (!a->delta || (rows16(a->delta, a->ld_delta, db) && rows16(a->res, a->ld_res, xb))) &&
+          (a->mode != FVB_NORM_GEMMA_RMS || aligned16(a->w)) &&
+          (a->mode != FVB_NORM_ADA_RMS || (aligned16(a->mod) && a->dim % 4 == 0));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int delta = !a->delta ? fvb::n8::DELTA_NONE
+                              : (a->delta_f32 ? fvb::n8::DELTA_F32 : fvb::n8::DELTA_BF16);
+  if (a->x_f32) return launch_norm_fp8<float>(d, delta, a->rows, st);
+  return launch_norm_fp8<bf16>(d, delta, a->rows, st);
+}
+
+int fvb_gemm_fp8(const fvb_gemm_fp8_args* a, void* stream) {
+  if (!a) return fail(FVB_ERR_INVALID_ARG, "args is NULL");
+  if (a->m < 0 || a->n <= 0 || a->k <= 0)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_gemm_fp8: bad shape %d x %d x %d", a->m, a->n, a->k);
+  if (a->epilogue != FVB_EPI_BF16 && a->epilogue != FVB_EPI_F32_STORE &&
+      a->epilogue != FVB_EPI_GEGLU)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_gemm_fp8: bad epilogue %d", a->epilogue);
+  if (a->epilogue == FVB_EPI_GEGLU && a->n % 2)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_gemm_fp8: GEGLU needs an even feature count");
+  if (!a->a || !a->a_scale || !a->b || !a->b_scale || !a->out)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_gemm_fp8: NULL operand");
+  const int groups = (a->k + 127) / 128;
+  const int nf = a->epilogue == FVB_EPI_GEGLU ? a->n / 2 : a->n;
+  if (a->lda < a->k || a->ldb < a->k || a->ld_as < groups || a->ld_bs < groups || a->ldo < nf)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_gemm_fp8: a row stride is shorter than its row");
+  if (!aligned16(a->a) || !aligned16(a->b) || a->lda % 16 || a->ldb % 16)
+    return fail(FVB_ERR_INVALID_ARG,
+                "fvb_gemm_fp8: operands must be 16B aligned with row strides in multiples of 16");
+  if (a->m == 0) return FVB_OK;
+  const bool swap = a->m <= 64;
+  int bn = 128;
+  if (swap) bn = a->m <= 16 ? 16 : (a->m <= 32 ? 32 : 64);
+  const int m_side = swap ? a->n : a->m, n_side = swap ? a->m : a->n;
+  const int m_tiles = (m_side + 127) / 128, n_tiles = (n_side + bn - 1) / bn;
+  const int64_t tiles = (int64_t)m_tiles * n_tiles;
+  const int sms = sm_count();
+  int cl = 1;
+  while (cl < 8 && tiles * cl * 2 <= sms + sms / 4 && cl * 2 <= groups) cl *= 2;
+  if (tiles * cl > INT32_MAX)
+    return fail(FVB_ERR_UNSUPPORTED, "fvb_gemm_fp8: too many tiles");
+  CUtensorMap ma, mb;
+  int r = swap ? make_map_u8(&ma, a->b, a->n, a->k, a->ldb, 128)
+               : make_map_u8(&ma, a->a, a->m, a->k, a->lda, 128);
+  if (!r) r = swap ? make_map_u8(&mb, a->a, a->m, a->k, a->lda, bn)
+                   : make_map_u8(&mb, a->b, a->n, a->k, a->ldb, bn);
+  if (r) return r;
+  fvb::g8::Dev d;
+  d.m = a->m; d.n = a->n; d.k = a->k;
+  d.groups = groups; d.m_tiles = m_tiles; d.cl = cl;
+  d.sa = a->a_scale; d.ld_sa = a->ld_as;
+  d.sb = a->b_scale; d.ld_sb = a->ld_bs;
+  d.out = a->out; d.ldo = a->ldo;
+  const int ob = a->epilogue == FVB_EPI_F32_STORE ? 16 : (a->epilogue == FVB_EPI_BF16 ? 8 : 4);
+  const int eb = a->epilogue == FVB_EPI_F32_STORE ? 4 : 2;
+  d.vec_out = aligned(a->out, ob) && a->ldo * eb % ob == 0;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (!swap) return launch_gemm_fp8<128, false>(a->epilogue, ma, mb, d, (int)tiles, st);
+  if (bn == 16) return launch_gemm_fp8<16, true>(a->epilogue, ma, mb, d, (int)tiles, st);
+  if (bn == 32) return launch_gemm_fp8<32, true>(a->epilogue, ma, mb, d, (int)tiles, st);
+  return launch_gemm_fp8<64, true>(a->epilogue, ma, mb, d, (int)tiles, st);
+}
+
+int fvb_paged_append(const fvb_paged_append_args* a, void* stream) {
+  if (!a) return fail(FVB_ERR_INVALID_ARG, "args is NULL");
+  if (a->tokens < 0 || a->heads < 0 || a->kv_heads <= 0 || a->head_dim <= 0 || a->head_dim % 2)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_paged_append: bad shape");
+  if (a->page_size <= 0 || a->n_pages < 0)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_paged_append: bad cache shape");
+  if (!a->k || !a->v || !a->k_cache || !a->v_cache || !a->slots)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_paged_append: NULL operand");
+  if (a->heads > 0 && (!a->q || !a->q_out))
+    return fail(FVB_ERR_INVALID_ARG, "fvb_paged_append: queries need q and q_out");
+  if (a->rope_cs && (!a->positions || a->max_pos <= 0 || !aligned(a->rope_cs, 8)))
+    return fail(FVB_ERR_INVALID_ARG, "fvb_paged_append: rope_cs needs positions and max_pos");
+  if (a->tokens == 0) return FVB_OK;
+  fvb::paged::AppendDev d;
+  d.q = (const bf16*)a->q; d.q_rs = a->q_row_stride; d.q_hs = a->q_head_stride;
+  d.k = (const bf16*)a->k; d.k_rs = a->k_row_stride; d.k_hs = a->k_head_stride;
+  d.v = (const bf16*)a->v; d.v_rs = a->v_row_stride; d.v_hs = a->v_head_stride;
+  d.q_out = (bf16*)a->q_out; d.qo_rs = a->q_out_row_stride; d.qo_hs = a->q_out_head_stride;
+  d.k_cache = (bf16*)a->k_cache; d.v_cache = (bf16*)a->v_cache;
+  d.kc_ps = a->kc_page_stride; d.kc_rs = a->kc_row_stride; d.kc_hs = a->kc_head_stride;
+  d.vc_ps = a->vc_page_stride; d.vc_rs = a->vc_row_stride; d.vc_hs = a->vc_head_stride;
+  d.slots = a->slots; d.positions = a->positions; d.rope_cs = a->rope_cs;
+  d.tokens = a->tokens; d.heads = a->heads; d.kv_heads = a->kv_heads; d.dim = a->head_dim;
+  d.page_size = a->page_size; d.max_pos = a->max_pos; d.interleaved = a->rope_interleaved;
+  d.n_slots = (long long)a->n_pages * a->page_size;
+  bool vec = a->head_dim % 16 == 0 && (!a->rope_cs || aligned16(a->rope_cs));
+  const void* ptrs[] = {a->q, a->k, a->v, a->q_out, a->k_cache, a->v_cache};
+  for (const void* p : ptrs) vec = vec && aligned16(p);
+  const int64_t strides[] = {d.q_rs, d.q_hs, d.k_rs, d.k_hs, d.v_rs, d.v_hs, d.qo_rs, d.qo_hs,
+                             d.kc_ps, d.kc_rs, d.kc_hs, d.vc_ps, d.vc_rs, d.vc_hs};
+  for (int i = a->heads > 0 ? 0 : 2; i < 14; ++i)
+    if (a->heads > 0 || (i != 6 && i != 7)) vec = vec && strides[i] % 8 == 0;
+  const int64_t per_token = (int64_t)(a->heads + 2 * a->kv_heads) * (a->head_dim / (vec ? 16 : 2));
+  const int64_t blocks = (per_token * a->tokens + 255) / 256;
+  if (per_token > INT32_MAX || blocks > INT32_MAX)
+    return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_append: too many rows");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return launch_k("fvb_paged_append",
+                  vec ? fvb::paged::append_kernel<true> : fvb::paged::append_kernel<false>,
+                  dim3((unsigned)blocks), dim3(256), 0, st, d);
+}
+
+int64_t fvb_paged_attention_workspace_bytes(const fvb_paged_attn_args* a) {
+  AttendShape s;
+  if (attend_prepare(a, &s)) return -1;
+  return s.bytes;
+}
+
+int fvb_paged_attention(const fvb_paged_attn_args* a, void* stream) {
+  AttendShape s;
+  int r = attend_prepare(a, &s);
+  if (r) return r;
+  if (!a->q || !a->k_cache || !a->v_cache || !a->page_table || !a->seq_lens || !a->out)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_paged_attention: NULL operand");
+  if (a->n_pages < 0 || a->page_size <= 0 || a->max_pages < 0 || a->ld_table < a->max_pages)
+    return fail(FVB_ERR_INVALID_ARG, "fvb_paged_attention: bad cache shape");
+  const int64_t max_len = (int64_t)a->max_pages * a->page_size;
+  if (max_len > INT32_MAX - 64)
+    return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attention: %lld keys a sequence",
+                (long long)max_len);
+  const int64_t s8[] = {a->kc_page_stride, a->kc_row_stride, a->kc_head_stride,
+                        a->vc_page_stride, a->vc_row_stride, a->vc_head_stride};
+  bool ok = aligned16(a->k_cache) && aligned16(a->v_cache);
+  for (int64_t v : s8) ok = ok && v % 8 == 0;
+  if (!ok)
+    return fail(FVB_ERR_INVALID_ARG,
+                "fvb_paged_attention: cache rows must be 16B aligned (strides in multiples of 8)");
+  if (!aligned(a->q, 4) || a->q_row_stride % 2 || a->q_head_stride % 2 || !aligned(a->out, 8) ||
+      a->out_row_stride % 4 || a->out_head_stride % 4)
+    return fail(FVB_ERR_INVALID_ARG,
+                "fvb_paged_attention: q needs 4-byte, out 8-byte aligned rows");
+  if (!a->workspace || a->workspace_bytes < s.bytes || !aligned16(a->workspace))
+    return fail(FVB_ERR_WORKSPACE, "fvb_paged_attention: workspace needs %lld bytes",
+                (long long)s.bytes);
+  if (a->batch == 0) return FVB_OK;
+  fvb::paged::AttendDev d;
+  d.q = (const bf16*)a->q; d.q_rs = a->q_row_stride; d.q_hs = a->q_head_stride;
+  d.k = (const bf16*)a->k_cache; d.k_ps = s8[0]; d.k_rs = s8[1]; d.k_hs = s8[2];
+  d.v = (const bf16*)a->v_cache; d.v_ps = s8[3]; d.v_rs = s8[4]; d.v_hs = s8[5];
+  d.o = (bf16*)a->out; d.o_rs = a->out_row_stride; d.o_hs = a->out_head_stride;
+  d.lse = a->lse; d.lse_rs = a->lse_row_stride;
+  d.table = a->page_table; d.ld_table = a->ld_table; d.lens = a->seq_lens;
+  d.batch = a->batch; d.heads = a->heads; d.kv_heads = a->kv_heads;
+  d.group = a->heads / a->kv_heads; d.head_blocks = s.head_blocks;
+  // without a page no key can be read, so every length is taken as 0
+  d.n_pages = a->n_pages; d.page_size = a->page_size;
+  d.max_len = a->n_pages > 0 ? (int)max_len : 0;
+  d.scale_log2 = a->scale * 1.4426950408889634f;
+  d.arrivals = (int*)a->workspace;
+  d.part_o = (float*)((char*)a->workspace + s.off_o);
+  d.part_ml = (float*)((char*)a->workspace + s.off_ml);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (a->head_dim == 256)
+    return s.nt == 1 ? launch_attend<256, 1>(d, s.ctas, st) : launch_attend<256, 2>(d, s.ctas, st);
+  if (a->head_dim == 128)
+    return s.nt == 1 ? launch_attend<128, 1>(d, s.ctas, st) : launch_attend<128, 2>(d, s.ctas, st);
+  return s.nt == 1 ? launch_attend<64, 1>(d, s.ctas, st) : launch_attend<64, 2>(d, s.ctas, st);
+}
+
+}  // extern "C"

@@ -8,8 +8,11 @@
 // (fluxvla/ops/cuda/matmul_bias/src/matmul_bias_forward.cpp:21-60).
 // Nothing here allocates; every output is caller-allocated.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <cstring>
 #include <sstream>
 #include <stdexcept>
 #include <string>
@@ -162,6 +165,249 @@ void small_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& ou
         "fvb_small_linear");
 }
 
+// ---- operators that serve several requests at once.  Their tensors may lie on
+// any device: the call runs on that device and its current stream.
+
+int64_t strided(const at::Tensor& t, at::ScalarType dt, int64_t dims, const char* name) {
+  require(t.scalar_type() == dt, name, ": expected ", dt, ", got ", t.scalar_type());
+  require(t.is_cuda(), name, ": must be a CUDA tensor");
+  require(t.dim() == dims && (t.stride(dims - 1) == 1 || t.size(dims - 1) <= 1), name,
+          ": expected ", dims, " dimensions, the last one contiguous");
+  return dims == 2 && t.size(0) <= 1 ? std::max(t.stride(0), t.size(1)) : t.stride(0);
+}
+
+void same_device(const at::Tensor& a, const at::Tensor& b, const char* name) {
+  require(a.device() == b.device(), name, ": on ", b.device(), ", expected ", a.device());
+}
+
+int32_t i32(int64_t v, const char* name) {
+  require(v >= 0 && v <= INT32_MAX, name, ": ", v, " is out of range");
+  return (int32_t)v;
+}
+
+bool f32_or_bf16(const at::Tensor& t, const char* name) {
+  require(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name,
+          ": expected float32 or bfloat16, got ", t.scalar_type());
+  return t.scalar_type() == at::kFloat;
+}
+
+void norm_fp8(int64_t mode, const at::Tensor& x, const at::Tensor& q, const at::Tensor& scales,
+              const OptT& delta, const OptT& res, const OptT& w, const OptT& mod, double eps) {
+  fvb_norm_fp8_args a;
+  memset(&a, 0, sizeof(a));
+  a.mode = (int32_t)mode;
+  a.x_f32 = f32_or_bf16(x, "x");
+  a.ld_x = strided(x, x.scalar_type(), 2, "x");
+  a.rows = i32(x.size(0), "rows");
+  a.dim = i32(x.size(1), "dim");
+  a.ld_q = strided(q, at::kFloat8_e4m3fn, 2, "out");
+  a.ld_scales = strided(scales, at::kFloat, 2, "scales");
+  require(q.sizes() == x.sizes(), "out: expected ", x.sizes(), ", got ", q.sizes());
+  require(scales.size(0) == a.rows && scales.size(1) == (a.dim + 127) / 128,
+          "scales: expected [", a.rows, ", ", (a.dim + 127) / 128, "], got ", scales.sizes());
+  same_device(x, q, "out");
+  same_device(x, scales, "scales");
+  require(delta.has_value() == res.has_value(), "delta and res come together");
+  if (delta.has_value()) {
+    a.delta_f32 = f32_or_bf16(*delta, "delta");
+    a.ld_delta = strided(*delta, delta->scalar_type(), 2, "delta");
+    a.ld_res = strided(*res, x.scalar_type(), 2, "res");
+    require(delta->sizes() == x.sizes() && res->sizes() == x.sizes(),
+            "delta and res: expected ", x.sizes(), ", got ", delta->sizes(), " and ",
+            res->sizes());
+    same_device(x, *delta, "delta");
+    same_device(x, *res, "res");
+    a.delta = delta->data_ptr();
+    a.res = res->data_ptr();
+  }
+  if (w.has_value()) {
+    require(w->scalar_type() == at::kBFloat16 && w->is_contiguous() && w->numel() == a.dim,
+            "w: expected ", a.dim, " contiguous bfloat16 values");
+    same_device(x, *w, "w");
+    a.w = w->data_ptr();
+  }
+  if (mod.has_value()) {
+    require(mod->scalar_type() == at::kFloat && mod->is_contiguous() && mod->numel() == 2 * a.dim,
+            "mod: expected ", 2 * (int64_t)a.dim, " contiguous float32 values");
+    same_device(x, *mod, "mod");
+    a.mod = mod->data_ptr<float>();
+  }
+  a.x = x.data_ptr();
+  a.q = q.data_ptr();
+  a.scales = scales.data_ptr<float>();
+  a.eps = eps;
+  if (a.rows == 0) return;
+  c10::cuda::CUDAGuard guard(x.device());
+  check(fvb_norm_fp8(&a, stream_ptr()), "fvb_norm_fp8");
+}
+
+void gemm_fp8(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b,
+              const at::Tensor& b_scale, const at::Tensor& out, int64_t epilogue) {
+  fvb_gemm_fp8_args g;
+  memset(&g, 0, sizeof(g));
+  g.lda = strided(a, at::kFloat8_e4m3fn, 2, "a");
+  g.ldb = strided(b, at::kFloat8_e4m3fn, 2, "b");
+  g.m = i32(a.size(0), "m");
+  g.n = i32(b.size(0), "n");
+  g.k = i32(a.size(1), "k");
+  require(b.size(1) == g.k, "K mismatch ", a.sizes(), " ", b.sizes());
+  const int64_t groups = (g.k + 127) / 128;
+  g.ld_as = strided(a_scale, at::kFloat, 2, "a_scale");
+  g.ld_bs = strided(b_scale, at::kFloat, 2, "b_scale");
+  require(a_scale.size(0) == g.m && a_scale.size(1) == groups, "a_scale: expected [", g.m, ", ",
+          groups, "], got ", a_scale.sizes());
+  require(b_scale.size(0) == (g.n + 127) / 128 && b_scale.size(1) == groups,
+          "b_scale: expected [", (g.n + 127) / 128, ", ", groups, "], got ", b_scale.sizes());
+  const bool f32 = epilogue == FVB_EPI_F32_STORE;
+  g.ldo = strided(out, f32 ? at::kFloat : at::kBFloat16, 2, "out");
+  const int64_t nf = epilogue == FVB_EPI_GEGLU ? g.n / 2 : g.n;
+  require(out.size(0) == g.m && out.size(1) == nf, "out: expected [", g.m, ", ", nf, "], got ",
+          out.sizes());
+  same_device(a, a_scale, "a_scale");
+  same_device(a, b, "b");
+  same_device(a, b_scale, "b_scale");
+  same_device(a, out, "out");
+  // a single row has no stride of its own to be aligned
+  if (g.m == 1) g.lda = (g.lda + 15) / 16 * 16;
+  if (g.n == 1) g.ldb = (g.ldb + 15) / 16 * 16;
+  g.a = a.data_ptr();
+  g.a_scale = a_scale.data_ptr<float>();
+  g.b = b.data_ptr();
+  g.b_scale = b_scale.data_ptr<float>();
+  g.out = out.data_ptr();
+  g.epilogue = (int32_t)epilogue;
+  if (g.m == 0) return;
+  c10::cuda::CUDAGuard guard(a.device());
+  check(fvb_gemm_fp8(&g, stream_ptr()), "fvb_gemm_fp8");
+}
+
+// a cache [pages, page_size, kv_heads, dim] and its strides
+void cache_strides(const at::Tensor& c, const char* name, int64_t* page, int64_t* row,
+                   int64_t* head) {
+  strided(c, at::kBFloat16, 4, name);
+  *page = c.stride(0);
+  *row = c.stride(1);
+  *head = c.stride(2);
+}
+
+int32_t* int_vector(const at::Tensor& t, int64_t n, const char* name) {
+  require(t.scalar_type() == at::kInt && t.is_cuda() && t.is_contiguous() && t.numel() == n, name,
+          ": expected ", n, " contiguous int32 values on the GPU");
+  return t.data_ptr<int32_t>();
+}
+
+void paged_append(const OptT& q, const at::Tensor& k, const at::Tensor& v,
+                  const at::Tensor& slots, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                  const OptT& q_out, const OptT& positions, const OptT& rope_cs,
+                  bool rope_interleaved) {
+  fvb_paged_append_args a;
+  memset(&a, 0, sizeof(a));
+  a.k_row_stride = strided(k, at::kBFloat16, 3, "k");
+  a.v_row_stride = strided(v, at::kBFloat16, 3, "v");
+  a.k_head_stride = k.stride(1);
+  a.v_head_stride = v.stride(1);
+  a.tokens = i32(k.size(0), "tokens");
+  a.kv_heads = i32(k.size(1), "kv_heads");
+  a.head_dim = i32(k.size(2), "head_dim");
+  require(v.sizes() == k.sizes(), "v: expected ", k.sizes(), ", got ", v.sizes());
+  cache_strides(k_cache, "k_cache", &a.kc_page_stride, &a.kc_row_stride, &a.kc_head_stride);
+  cache_strides(v_cache, "v_cache", &a.vc_page_stride, &a.vc_row_stride, &a.vc_head_stride);
+  require(k_cache.size(2) == a.kv_heads && k_cache.size(3) == a.head_dim &&
+              v_cache.sizes() == k_cache.sizes(),
+          "caches: expected [pages, page_size, ", a.kv_heads, ", ", a.head_dim, "], got ",
+          k_cache.sizes(), " and ", v_cache.sizes());
+  a.n_pages = i32(k_cache.size(0), "pages");
+  a.page_size = i32(k_cache.size(1), "page_size");
+  a.slots = int_vector(slots, a.tokens, "slots");
+  for (const at::Tensor* t : {&v, &slots, &k_cache, &v_cache}) same_device(k, *t, "operand");
+  require(q.has_value() == q_out.has_value(), "q and q_out come together");
+  if (q.has_value()) {
+    a.q_row_stride = strided(*q, at::kBFloat16, 3, "q");
+    a.q_out_row_stride = strided(*q_out, at::kBFloat16, 3, "q_out");
+    a.q_head_stride = q->stride(1);
+    a.q_out_head_stride = q_out->stride(1);
+    a.heads = i32(q->size(1), "heads");
+    require(q->size(0) == a.tokens && q->size(2) == a.head_dim && q_out->sizes() == q->sizes(),
+            "q and q_out: expected [", a.tokens, ", heads, ", a.head_dim, "], got ", q->sizes(),
+            " and ", q_out->sizes());
+    same_device(k, *q, "q");
+    same_device(k, *q_out, "q_out");
+    a.q = q->data_ptr();
+    a.q_out = q_out->data_ptr();
+  }
+  require(positions.has_value() == rope_cs.has_value(), "positions and rope_cs come together");
+  if (rope_cs.has_value()) {
+    require(rope_cs->scalar_type() == at::kFloat && rope_cs->is_contiguous() &&
+                rope_cs->dim() == 3 && rope_cs->size(0) > 0 &&
+                rope_cs->size(1) * 2 == a.head_dim && rope_cs->size(2) == 2,
+            "rope_cs: expected contiguous float32 [positions, head_dim / 2, 2]");
+    same_device(k, *rope_cs, "rope_cs");
+    same_device(k, *positions, "positions");
+    a.rope_cs = rope_cs->data_ptr<float>();
+    a.max_pos = i32(rope_cs->size(0), "positions");
+    a.positions = int_vector(*positions, a.tokens, "positions");
+  }
+  a.rope_interleaved = rope_interleaved;
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = v_cache.data_ptr();
+  if (a.tokens == 0) return;
+  c10::cuda::CUDAGuard guard(k.device());
+  check(fvb_paged_append(&a, stream_ptr()), "fvb_paged_append");
+}
+
+void paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                     const at::Tensor& page_table, const at::Tensor& seq_lens,
+                     const at::Tensor& out, double scale, const OptT& lse,
+                     const at::Tensor& workspace) {
+  fvb_paged_attn_args a;
+  memset(&a, 0, sizeof(a));
+  a.q_row_stride = strided(q, at::kBFloat16, 3, "q");
+  a.out_row_stride = strided(out, at::kBFloat16, 3, "out");
+  a.q_head_stride = q.stride(1);
+  a.out_head_stride = out.stride(1);
+  require(out.sizes() == q.sizes(), "out: expected ", q.sizes(), ", got ", out.sizes());
+  a.batch = i32(q.size(0), "batch");
+  a.heads = i32(q.size(1), "heads");
+  a.head_dim = i32(q.size(2), "head_dim");
+  cache_strides(k_cache, "k_cache", &a.kc_page_stride, &a.kc_row_stride, &a.kc_head_stride);
+  cache_strides(v_cache, "v_cache", &a.vc_page_stride, &a.vc_row_stride, &a.vc_head_stride);
+  require(k_cache.size(3) == a.head_dim && v_cache.sizes() == k_cache.sizes(),
+          "caches: expected [pages, page_size, kv_heads, ", a.head_dim, "], got ",
+          k_cache.sizes(), " and ", v_cache.sizes());
+  a.n_pages = i32(k_cache.size(0), "pages");
+  a.page_size = i32(k_cache.size(1), "page_size");
+  a.kv_heads = i32(k_cache.size(2), "kv_heads");
+  a.ld_table = strided(page_table, at::kInt, 2, "page_table");
+  require(page_table.size(0) == a.batch, "page_table: expected ", a.batch, " rows, got ",
+          page_table.sizes());
+  a.max_pages = i32(page_table.size(1), "page_table columns");
+  a.seq_lens = int_vector(seq_lens, a.batch, "seq_lens");
+  require(workspace.is_cuda() && workspace.is_contiguous(),
+          "workspace: expected a contiguous CUDA tensor");
+  for (const at::Tensor* t : {&k_cache, &v_cache, &page_table, &seq_lens, &out, &workspace})
+    same_device(q, *t, "operand");
+  if (lse.has_value()) {
+    a.lse_row_stride = strided(*lse, at::kFloat, 2, "lse");
+    require(lse->size(0) == a.batch && lse->size(1) == a.heads, "lse: expected [", a.batch, ", ",
+            a.heads, "], got ", lse->sizes());
+    same_device(q, *lse, "lse");
+    a.lse = lse->data_ptr<float>();
+  }
+  a.q = q.data_ptr();
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = v_cache.data_ptr();
+  a.page_table = page_table.data_ptr<int32_t>();
+  a.out = out.data_ptr();
+  a.scale = (float)scale;
+  a.workspace = workspace.data_ptr();
+  a.workspace_bytes = workspace.numel() * workspace.element_size();
+  if (a.batch == 0) return;
+  c10::cuda::CUDAGuard guard(q.device());
+  check(fvb_paged_attention(&a, stream_ptr()), "fvb_paged_attention");
+}
+
 // A C-ABI error surfaced as a Python exception without touching the GPU
 // (fvb_get_device_status rejects a NULL pointer): used by the tests.
 void error_path_probe() { check(fvb_get_device_status(nullptr, 0), "fvb_get_device_status"); }
@@ -175,5 +421,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("norm_bf16", &norm_bf16);
   m.def("softmax_rows", &softmax_rows);
   m.def("small_linear", &small_linear);
+  m.def("norm_fp8", &norm_fp8);
+  m.def("gemm_fp8", &gemm_fp8);
+  m.def("paged_append", &paged_append);
+  m.def("paged_attention", &paged_attention);
   m.def("error_path_probe", &error_path_probe);
 }

@@ -19,7 +19,7 @@ import torch
 from . import _lib
 from ._lib import (ACT_NONE, EPI_BF16, EPI_F32_ACC, EPI_F32_STORE,
                    EPI_GEGLU, EPI_QKV_ROPE, AttnArgs, ExpertArgs, GemmArgs,
-                   check)
+                   PagedAttnArgs, check)
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -198,6 +198,68 @@ def small_linear(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *,
     """y = act(x @ w[:, :k]^T + bias); mode 0 store f32, 1 store bf16,
     2 out += alpha*y (f32)."""
     _C().small_linear(x, w, out, bias, act, mode, alpha, k or 0)
+
+
+def norm_fp8(mode: int, x: torch.Tensor, out: torch.Tensor,
+             scales: torch.Tensor, *, delta=None, res=None, w=None, mod=None,
+             eps: float = 1e-6) -> None:
+    """e4m3 codes of normalised rows, one f32 scale per 128 columns
+    (fvb_norm_fp8): ``res`` = x + delta if ``delta`` is given (``res`` may be
+    ``x``), then NORM_GEMMA_RMS (w), NORM_ADA_RMS (mod: scale | shift),
+    NORM_RMS or NORM_NONE, then ``out`` (float8_e4m3fn [rows, dim]) and
+    ``scales`` ([rows, ceil(dim / 128)]).  x: f32 or bf16 rows, delta
+    either."""
+    _C().norm_fp8(mode, x, out, scales, delta, res, w, mod, eps)
+
+
+def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
+             b_scale: torch.Tensor, out: torch.Tensor, *,
+             epilogue: int = EPI_BF16) -> None:
+    """out = (a * a_scale) @ (b * b_scale)^T of float8_e4m3fn operands
+    (fvb_gemm_fp8): a [M, K] with a_scale [M, ceil(K / 128)] as norm_fp8 gives
+    them, b [N, K] with b_scale [ceil(N / 128), ceil(K / 128)] as
+    pack.quantize_blocks lays them out.  EPI_BF16, EPI_F32_STORE, or EPI_GEGLU
+    (rows of b packed by pack.pack_geglu, out [M, N / 2])."""
+    _C().gemm_fp8(a, a_scale, b, b_scale, out, epilogue)
+
+
+def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
+                 slots: torch.Tensor, k_cache: torch.Tensor,
+                 v_cache: torch.Tensor, *, q_out=None, positions=None,
+                 rope_cs=None, rope_interleaved: bool = False) -> None:
+    """Keys and values of new tokens into a paged cache, queries and keys
+    rotated by their positions (fvb_paged_append): q [T, heads, dim] (or None)
+    -> q_out, k and v [T, kv_heads, dim] -> [pages, page_size, kv_heads, dim]
+    at ``slots`` (int32, page * page_size + row; negative: not cached).
+    ``rope_cs`` [max_pos, dim / 2, 2] as pack.rope_table, None: no rotation."""
+    _C().paged_append(q, k, v, slots, k_cache, v_cache, q_out, positions,
+                      rope_cs, rope_interleaved)
+
+
+def paged_attention_workspace_bytes(heads: int, kv_heads: int,
+                                    head_dim: int) -> int:
+    """Bytes of the (zeroed) workspace of paged_attention on the current
+    device, for any batch and any lengths."""
+    a = PagedAttnArgs(heads=heads, kv_heads=kv_heads, head_dim=head_dim)
+    n = _lib.lib().fvb_paged_attention_workspace_bytes(C.byref(a))
+    if n < 0:
+        check(1)
+    return int(n)
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor,
+                    v_cache: torch.Tensor, page_table: torch.Tensor,
+                    seq_lens: torch.Tensor, out: torch.Tensor, *,
+                    scale: float, workspace: torch.Tensor,
+                    lse: Optional[torch.Tensor] = None) -> None:
+    """One new token of each sequence over its pages (fvb_paged_attention):
+    q and out [batch, heads, dim], page_table int32 [batch, pages], seq_lens
+    int32 [batch] (the new token's key included), lse f32 [batch, heads] or
+    None.  ``workspace``: a zeroed uint8 tensor of
+    paged_attention_workspace_bytes(...); calls that share one must not
+    overlap on the GPU."""
+    _C().paged_attention(q, k_cache, v_cache, page_table, seq_lens, out,
+                         scale, lse, workspace)
 
 
 def probe_wait_timeout(limit_s: float = 0.05) -> bool:

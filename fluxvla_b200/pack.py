@@ -50,3 +50,18 @@ def rope_table(max_pos: int, head_dim: int, theta: float = 10000.0,
                            .float() / head_dim))
     f = torch.arange(max_pos, dtype=torch.int64).float()[:, None] * inv
     return torch.stack([f.cos(), f.sin()], dim=-1).contiguous().to(device)
+
+
+def quantize_blocks(w: torch.Tensor):
+    """[N, K] weights -> (float8_e4m3fn codes [N, K], f32 scales
+    [ceil(N/128), ceil(K/128)]): one scale per 128 x 128 block, max |w| of the
+    block / 448, as ops.gemm_fp8 reads them.  Rows packed for an epilogue
+    (pack_geglu) are packed before."""
+    n, k = w.shape
+    gn, gk = -(-n // 128), -(-k // 128)
+    x = w.new_zeros((gn * 128, gk * 128), dtype=torch.float64)
+    x[:n, :k] = w
+    x = x.view(gn, 128, gk, 128)
+    s = (x.abs().amax(dim=(1, 3)).clamp(min=2.0 ** -60) / 448.0).float()
+    t = (x / s.double()[:, None, :, None]).view(gn * 128, gk * 128)[:n, :k]
+    return t.float().clamp(-448.0, 448.0).to(torch.float8_e4m3fn), s

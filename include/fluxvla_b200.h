@@ -61,6 +61,7 @@ extern "C" {
 #define FVB_NORM_LAYER 2     /* (x-mean)*rsqrt(var+eps)*w + b              */
 #define FVB_NORM_RMS 3       /* x*rsqrt(mean(x^2)+eps), no weight (fvb_norm_bf16) */
 #define FVB_NORM_ADA_STYLE 4 /* x*rsqrt(mean(x^2)+eps)*(1+scale)+shift, gate out  */
+#define FVB_NORM_NONE 5      /* x itself (fvb_norm_fp8: codes without a norm)      */
 
 typedef struct fvb_gemm_args {
   /* C[M,N] = A[M,K] * B[N,K]^T, bf16 operands, f32 accumulation.         */
@@ -303,6 +304,149 @@ int fvb_norm_bf16(int32_t mode, const void* x, int64_t ld_in, void* out,
                   int64_t ld_out, int32_t rows, int32_t dim, const void* w,
                   const void* b, const void* style, void* gate_out,
                   int64_t ld_gate, float eps, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Operators of a decoder layer that serves several requests at once: e4m3
+ * products with block scales and the norm that feeds them, and a key-value
+ * cache in pages.  The reference has no counterpart: its request loop
+ * (fluxvla/serving/zmq_server.py) runs one request at a time over a
+ * contiguous cache with bf16 weights.
+ * ------------------------------------------------------------------------- */
+
+/* Largest row of fvb_norm_fp8 with a norm (FVB_NORM_NONE has no limit). */
+#define FVB_NORM_FP8_MAX_DIM 16384
+
+typedef struct fvb_norm_fp8_args {
+  int32_t mode; /* FVB_NORM_GEMMA_RMS (w), FVB_NORM_ADA_RMS (mod), FVB_NORM_RMS,
+                 * FVB_NORM_NONE */
+  int32_t rows, dim;
+  const void* x; /* bf16 or f32 (x_f32 = 1) [rows, ld_x] */
+  int64_t ld_x;
+  int32_t x_f32;
+  const void* delta; /* bf16 or f32 (delta_f32 = 1) [rows, ld_delta] or NULL */
+  int64_t ld_delta;
+  int32_t delta_f32;
+  void* res; /* with delta: the type of x [rows, ld_res]; may be x */
+  int64_t ld_res;
+  const void* w;    /* bf16 [dim] */
+  const float* mod; /* [2*dim] (scale | shift) */
+  double eps;
+  void* q; /* e4m3 [rows, ld_q] */
+  int64_t ld_q;
+  float* scales; /* [rows, ld_scales], ceil(dim / 128) of each row written */
+  int64_t ld_scales;
+} fvb_norm_fp8_args;
+
+/* Residual addition, norm and e4m3 codes of rows, what fvb_gemm_fp8 reads:
+ *   h = round(x + delta)           -> res (x's type; h = x without delta)
+ *   y = h * rsqrt(mean(h^2) + eps) * (1 + w) | * (1 + scale) + shift | h
+ *   scale of 128 columns = max(max |y|, 2^-60) / 448, rounded to f32
+ *   code = y / scale rounded to e4m3 (ties to even)
+ * Between its inputs and the two roundings nothing is rounded to fewer than
+ * 64 bits.  A NaN gets the NaN code and does not count for its group's
+ * scale; a group that holds an infinity has an infinite scale and decodes as
+ * NaN.  rows = 0 is a call that does nothing.  Rows that are 16-byte aligned
+ * (x, delta, res) and 8-byte aligned (q) are moved in vectors, others value by
+ * value.                                                                    */
+int fvb_norm_fp8(const fvb_norm_fp8_args* args, void* stream);
+
+typedef struct fvb_gemm_fp8_args {
+  const void* a; /* e4m3 [m, lda] token rows; 16-byte aligned, lda % 16 == 0 */
+  int64_t lda;
+  const float* a_scale; /* [m, ld_as]: one scale per 128 columns of a row */
+  int64_t ld_as;
+  const void* b; /* e4m3 [n, ldb] weights, nn.Linear layout; aligned like a */
+  int64_t ldb;
+  const float* b_scale; /* [ceil(n/128), ld_bs]: one scale per 128 x 128 block */
+  int64_t ld_bs;
+  int32_t m, n, k;
+  int32_t epilogue; /* FVB_EPI_BF16, FVB_EPI_F32_STORE, FVB_EPI_GEGLU */
+  void* out;        /* bf16 or f32 [m, ldo]; GEGLU: bf16 [m, n/2] */
+  int64_t ldo;
+} fvb_gemm_fp8_args;
+
+/* out[t, f] = sum over groups g of 128 columns of a_scale[t, g] *
+ * b_scale[f / 128, g] * (sum over k in g of a[t, k] * b[f, k]), accumulated
+ * in f32; GEGLU as in fvb_gemm (features 2i, 2i+1 are gate and up of output
+ * i).  k need not be a multiple of 128.  The sums have a fixed order: the same
+ * call gives the same bits.  m = 0 is a call that does nothing.             */
+int fvb_gemm_fp8(const fvb_gemm_fp8_args* args, void* stream);
+
+typedef struct fvb_paged_append_args {
+  /* Element (token t, head h, dim d) of q is q[t*q_row_stride +
+   * h*q_head_stride + d]; k, v and q_out alike (views of one packed
+   * projection will do).  q_out may be q.  heads = 0: keys and values only. */
+  const void* q;
+  int64_t q_row_stride, q_head_stride;
+  const void* k;
+  int64_t k_row_stride, k_head_stride;
+  const void* v;
+  int64_t v_row_stride, v_head_stride;
+  void* q_out;
+  int64_t q_out_row_stride, q_out_head_stride;
+  /* bf16 cache: element (page, row, head, d) at page*page_stride +
+   * row*row_stride + head*head_stride + d                                   */
+  void* k_cache;
+  int64_t kc_page_stride, kc_row_stride, kc_head_stride;
+  void* v_cache;
+  int64_t vc_page_stride, vc_row_stride, vc_head_stride;
+  int32_t n_pages, page_size;
+  const int32_t* slots; /* [tokens]: page * page_size + row; < 0: not cached */
+  const int32_t* positions; /* [tokens], with rope_cs */
+  const float* rope_cs;     /* [max_pos, head_dim/2, 2] (cos, sin) or NULL */
+  int32_t max_pos;
+  int32_t rope_interleaved; /* pairs (2i, 2i+1) instead of (i, i + head_dim/2) */
+  int32_t tokens, heads, kv_heads, head_dim; /* head_dim even */
+} fvb_paged_append_args;
+
+/* Rotates the new queries and keys by their positions (f32, rounded once to
+ * bf16) and writes keys and values to their slots of the cache; the rest of
+ * the cache is left as it is.  A token whose slot is negative (padding) is not
+ * cached; its queries are still rotated, or left alone if its position is
+ * outside the table too.  A slot past the cache, or a cached token's position
+ * outside the table, writes nothing and sets FVB_ERR_INVALID_ARG in the device
+ * status word.  Slots of one call are distinct: of two tokens with the same
+ * slot it is not defined which one's values stay.                           */
+int fvb_paged_append(const fvb_paged_append_args* args, void* stream);
+
+typedef struct fvb_paged_attn_args {
+  const void* q; /* bf16, element (sequence b, head h, d) by strides */
+  int64_t q_row_stride, q_head_stride;
+  const void* k_cache; /* bf16 pages as in fvb_paged_append; 16-byte rows */
+  int64_t kc_page_stride, kc_row_stride, kc_head_stride;
+  const void* v_cache;
+  int64_t vc_page_stride, vc_row_stride, vc_head_stride;
+  int32_t n_pages, page_size;
+  const int32_t* page_table; /* [batch, ld_table]: pages of each sequence */
+  int64_t ld_table;
+  int32_t max_pages;       /* columns of the table that may be read */
+  const int32_t* seq_lens; /* [batch] keys of each sequence, in device memory */
+  void* out;               /* bf16, by strides like q */
+  int64_t out_row_stride, out_head_stride;
+  float* lse; /* [batch, lse_row_stride]: log of the sum of exp, or NULL */
+  int64_t lse_row_stride;
+  int32_t batch, heads, kv_heads, head_dim; /* head_dim 64, 128 or 256 */
+  float scale;
+  void* workspace; /* fvb_paged_attention_workspace_bytes(); 16-byte aligned */
+  int64_t workspace_bytes;
+} fvb_paged_attn_args;
+
+/* Attention of one new token of each sequence (its key already appended) over
+ * the sequence's pages; query head h reads kv head h / (heads / kv_heads).
+ * One launch whatever the lengths are: they are read on the device, so a
+ * captured call follows them.  A length of 0 gives zeros and lse = -inf.
+ * Table entries past a sequence's last page are not read.  A length outside
+ * [0, max_pages * page_size] is clamped, a page outside the cache read as
+ * page 0, and either sets FVB_ERR_INVALID_ARG in the device status word.
+ *
+ * The workspace must be zero-filled before its first use and every call
+ * leaves it ready for the next, of any shape.  Calls that share one must not
+ * overlap on the GPU.  The partial sums of a sequence are joined in the order
+ * of its keys: the same call gives the same bits.                           */
+int fvb_paged_attention(const fvb_paged_attn_args* args, void* stream);
+/* Workspace bytes for this head_dim, heads and kv_heads on the current
+ * device; it does not grow with the batch or the lengths.                   */
+int64_t fvb_paged_attention_workspace_bytes(const fvb_paged_attn_args* args);
 
 /* Row softmax of materialised attention logits, for callers that keep the
  * reference's unfused attention (matmul_abT_scale -> softmax -> P.V):

@@ -1,0 +1,596 @@
+"""The serving operators (e4m3 norm and product, paged append and attention)
+against 64-bit restatements, at the sizes, strides and masks where they can go
+wrong; then a decoder layer of them, in order."""
+import math
+
+import pytest
+import torch
+
+from fluxvla_b200 import _lib, ops, pack
+from tests import serving_ref as R
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+E4M3 = torch.float8_e4m3fn
+BF16_HALF = 2.0 ** -8      # half a step, relative
+DEV = 'cuda'
+MODES = {'gemma': _lib.NORM_GEMMA_RMS, 'ada': _lib.NORM_ADA_RMS,
+         'rms': _lib.NORM_RMS, 'none': _lib.NORM_NONE}
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def randn(g, *shape, dt=F32):
+    return torch.randn(*shape, generator=g, device=DEV).to(dt)
+
+
+def values(q):
+    return q.to(F32).to(F64)
+
+
+# ---------------------------------------------------------------- norm_fp8
+def norm_inputs(g, rows, dim, mode, xt, dt):
+    x = randn(g, rows, dim) * (1 + 20 * (torch.rand(
+        dim, generator=g, device=DEV) > 0.97))
+    x = x.to(xt)
+    kw = {}
+    if dt is not None:
+        kw['delta'] = randn(g, rows, dim, dt=dt)
+    if mode == 'gemma':
+        kw['w'] = randn(g, dim, dt=BF16) * 0.3
+    if mode == 'ada':
+        kw['mod'] = randn(g, 2 * dim) * 0.3
+    return x, kw
+
+
+def check_norm(mode, x, kw, q, s, res=None):
+    """Codes, scales and residual are those of the formula: nothing is rounded
+    before them to fewer than 64 bits, so nothing may differ."""
+    h, q_ref, s_ref = R.norm_fp8(MODES[mode], x, **kw)
+    if 'delta' in kw:
+        assert torch.equal(res, h)
+    assert torch.equal(s, s_ref)
+    assert torch.equal(values(q), q_ref)
+
+
+@pytest.mark.parametrize('mode', list(MODES))
+@pytest.mark.parametrize('xt,dt', [(F32, BF16), (BF16, BF16), (F32, None),
+                                   (BF16, F32)])
+@pytest.mark.parametrize('rows,dim', [(1, 1), (1, 2048), (3, 127), (5, 129),
+                                      (64, 1024), (2, 1152), (7, 4304),
+                                      (2, 8192), (3, 16384), (130, 64)])
+def test_norm_fp8(mode, xt, dt, rows, dim):
+    g = gen(rows * 131 + dim)
+    x, kw = norm_inputs(g, rows, dim, mode, xt, dt)
+    q = torch.empty(rows, dim, dtype=E4M3, device=DEV)
+    s = torch.empty(rows, -(-dim // 128), device=DEV)
+    res = torch.empty_like(x) if dt is not None else None
+    ops.norm_fp8(MODES[mode], x, q, s, res=res, **kw)
+    check_norm(mode, x, kw, q, s, res)
+
+
+def test_norm_fp8_strides_in_place_and_beyond_the_norm_limit():
+    g = gen(1)
+    # views into wider buffers, odd offsets: value-by-value path; the columns
+    # around the views stay as they were
+    big = randn(g, 6, 301)
+    wide_q = torch.full((6, 305), 7, dtype=torch.uint8, device=DEV)
+    wide_s = torch.full((6, 5), 9.0, device=DEV)
+    x = big[:, 1:301]
+    kw = dict(delta=randn(g, 6, 300, dt=BF16), w=randn(g, 300, dt=BF16))
+    before = big.clone()
+    ref = before[:, 1:301]
+    q, s = wide_q.view(E4M3)[:, 3:303], wide_s[:, 1:4]
+    ops.norm_fp8(_lib.NORM_GEMMA_RMS, x, q, s, res=x, **kw)
+    check_norm('gemma', ref, kw, q, s, x)
+    assert torch.equal(big[:, 0], before[:, 0])
+    assert (wide_q[:, :3] == 7).all() and (wide_q[:, 303:] == 7).all()
+    assert (wide_s[:, 0] == 9).all() and (wide_s[:, 4] == 9).all()
+    # without a norm a row may be longer than the norms' limit
+    x = randn(g, 2, 20000, dt=BF16)
+    q = torch.empty(2, 20000, dtype=E4M3, device=DEV)
+    s = torch.empty(2, 157, device=DEV)
+    ops.norm_fp8(_lib.NORM_NONE, x, q, s)
+    check_norm('none', x, {}, q, s)
+
+
+def test_norm_fp8_values_on_the_borders_between_codes():
+    """Every border of the format, times a scale that is not a power of two,
+    and its neighbours: the even code, and the codes on either side."""
+    grid = R.e4m3_grid().float().to(DEV)
+    mid = (grid[1:] + grid[:-1]) / 2
+    for unit in (1.0, 3.0, 2.0 ** -20 * 5):
+        row = torch.zeros(5, 128, device=DEV)
+        flat = torch.cat([mid, torch.nextafter(mid, mid * 2),
+                          torch.nextafter(mid, mid * 0)]) * unit
+        # one slot in each group holds the largest value, which sets the scale
+        body = torch.zeros(row.shape[0] * 127, device=DEV)
+        body[:flat.numel()] = flat
+        row[:, 1:] = body.view(-1, 127)
+        row[:, 0] = -448.0 * unit
+        q = torch.empty(row.shape, dtype=E4M3, device=DEV)
+        s = torch.empty(row.shape[0], 1, device=DEV)
+        ops.norm_fp8(_lib.NORM_NONE, row, q, s)
+        check_norm('none', row, {}, q, s)
+
+
+def test_norm_fp8_zero_tiny_nan_and_infinite_rows():
+    x = torch.zeros(5, 256, device=DEV)
+    x[1] = 1e-30                      # below the smallest scale
+    x[2, 5] = math.nan
+    x[2, 6:] = 2.0
+    x[3, 200] = math.inf
+    x[3, :128] = 1.0
+    x[4] = 3e38
+    q = torch.empty(5, 256, dtype=E4M3, device=DEV)
+    s = torch.empty(5, 2, device=DEV)
+    ops.norm_fp8(_lib.NORM_NONE, x, q, s)
+    v = values(q) * s.to(F64).repeat_interleave(128, 1)
+    assert (v[0] == 0).all() and (v[1] == 0).all()
+    assert torch.isnan(v[2, 5]) and torch.isfinite(v[2, 6:]).all()
+    assert (v[2, 6:128] - 2).abs().max() <= 2.0 ** -23   # the scale's rounding
+    assert torch.isfinite(v[3, :128]).all() and torch.isnan(v[3, 128:]).all()
+    assert ((v[4] / 3e38 - 1).abs() <= 2.0 ** -22).all()
+    # a zero row through a norm: zeros, not NaN
+    w = torch.zeros(256, dtype=BF16, device=DEV)
+    ops.norm_fp8(_lib.NORM_GEMMA_RMS, x[:1], q[:1], s[:1], w=w)
+    assert (values(q[:1]) == 0).all()
+
+
+# ---------------------------------------------------------------- gemm_fp8
+def gemm_inputs(g, m, n, k):
+    x = randn(g, m, k)
+    a = torch.empty(m, k, dtype=E4M3, device=DEV)
+    sa = torch.empty(m, -(-k // 128), device=DEV)
+    ops.norm_fp8(_lib.NORM_NONE, x, a, sa)
+    b, sb = pack.quantize_blocks(randn(g, n, k) * k ** -0.5)
+    return a, sa, b, sb
+
+
+def check_gemm(out, a, sa, b, sb, epilogue):
+    """Each product of two e4m3 values is exact in f32; a group of 128 and the
+    sum over groups add at most 128 + groups roundings (2^-23 of the partial
+    sum where additions truncate), the two scales one each."""
+    c, mag = R.gemm_fp8(a, sa, b, sb)
+    err = mag * (128 + sa.shape[1] + 8 + 4) * 2.0 ** -23
+    if epilogue == _lib.EPI_GEGLU:
+        gate, up = c[:, 0::2], c[:, 1::2]
+        eg, eu = err[:, 0::2], err[:, 1::2]
+        ref = R.gelu(gate) * up
+        # |gelu'| <= 1.13; exp and the division add a few f32 roundings
+        err = 1.13 * eg * (up.abs() + eu) + R.gelu(gate).abs() * eu
+        err = err + 2.0 ** -18 * (ref.abs() + gate.abs() * up.abs() * 2.0 ** -6)
+    else:
+        ref = c
+    if out.dtype == BF16:
+        err = err + BF16_HALF * (ref.abs() + err)
+    bad = (out.to(F64) - ref).abs() > err
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist())
+
+
+EPIS = {'bf16': _lib.EPI_BF16, 'f32': _lib.EPI_F32_STORE,
+        'geglu': _lib.EPI_GEGLU}
+
+
+@pytest.mark.parametrize('epi', list(EPIS))
+@pytest.mark.parametrize('m,n,k', [
+    (1, 2, 1), (1, 128, 128), (1, 2560, 2048), (3, 130, 144), (16, 256, 300),
+    (17, 1152, 4304), (33, 254, 1000), (51, 1024, 4096), (64, 2048, 16384),
+    (65, 128, 256), (100, 514, 640), (128, 256, 128), (129, 130, 272),
+    (300, 1152, 1152), (816, 2560, 2048), (257, 4098, 1040)])
+def test_gemm_fp8(epi, m, n, k):
+    g = gen(m + 3 * n + 7 * k)
+    kp = -(-k // 16) * 16          # rows of 16-byte multiples
+    a, sa, b, sb = gemm_inputs(g, m, n, kp)
+    a, b = a[:, :k], b[:, :k]      # and a width that is none
+    cols = n // 2 if epi == 'geglu' else n
+    wide = torch.full((m + 2, cols + 8), 5.0, device=DEV,
+                      dtype=F32 if epi == 'f32' else BF16)
+    out = wide[1:m + 1, :cols]
+    ops.gemm_fp8(a, sa, b, sb, out, epilogue=EPIS[epi])
+    check_gemm(out, a, sa, b, sb, EPIS[epi])
+    assert (wide[0] == 5).all() and (wide[m + 1] == 5).all()
+    assert (wide[:, cols:] == 5).all()
+    again = torch.empty_like(out)
+    ops.gemm_fp8(a, sa, b, sb, again, epilogue=EPIS[epi])
+    assert torch.equal(again, out)
+    assert ops.device_status() == 0
+
+
+def test_gemm_fp8_nan_stays_in_its_row_and_column():
+    g = gen(5)
+    a, sa, b, sb = gemm_inputs(g, 70, 192, 256)
+    a.view(torch.uint8)[3, 9] = 0x7f
+    b.view(torch.uint8)[100, 200] = 0x7f
+    out = torch.empty(70, 192, device=DEV)
+    ops.gemm_fp8(a, sa, b, sb, out, epilogue=_lib.EPI_F32_STORE)
+    nan = torch.zeros(70, 192, dtype=torch.bool, device=DEV)
+    nan[3], nan[:, 100] = True, True
+    assert torch.equal(torch.isnan(out), nan)
+
+
+# ------------------------------------------------------------ paged_append
+def rope(max_pos, dim):
+    return pack.rope_table(max_pos, dim, device=DEV)
+
+
+@pytest.mark.parametrize('tokens,heads,kv,dim,page', [
+    (1, 8, 1, 256, 16), (51, 8, 1, 256, 48), (7, 4, 2, 64, 1),
+    (33, 6, 3, 128, 100), (5, 2, 1, 72, 8), (9, 3, 3, 10, 4), (2, 0, 2, 128, 32)])
+@pytest.mark.parametrize('interleaved', [False, True])
+def test_paged_append(tokens, heads, kv, dim, page, interleaved):
+    g = gen(tokens * 7 + dim)
+    qkv = randn(g, tokens, (heads + 2 * kv) * dim + 8, dt=BF16)[:, :-8]
+    rows = qkv.unflatten(1, (heads + 2 * kv, dim))
+    q, k, v = rows[:, :heads], rows[:, heads:heads + kv], rows[:, heads + kv:]
+    pages = -(-tokens // page) + 2
+    slots = torch.randperm(pages * page, generator=g, device=DEV)[:tokens]
+    slots = slots.to(torch.int32)
+    if tokens > 4:
+        slots[2] = -1
+        slots[4] = -100
+    pos = torch.randint(0, 500, (tokens,), generator=g, device=DEV,
+                        dtype=torch.int32)
+    table = rope(500, dim)
+    kc = randn(g, pages, page, kv, dim, dt=BF16)
+    vc = randn(g, pages, page, kv, dim, dt=BF16)
+    kc0, vc0 = kc.clone(), vc.clone()
+    q_out = torch.empty(tokens, heads, dim, dtype=BF16, device=DEV)
+    if heads:
+        ops.paged_append(q, k, v, slots, kc, vc, q_out=q_out, positions=pos,
+                         rope_cs=table, rope_interleaved=interleaved)
+    else:
+        ops.paged_append(None, k, v, slots, kc, vc, positions=pos,
+                         rope_cs=table, rope_interleaved=interleaved)
+
+    def near(got, x):
+        # two products and a sum in f32, then one rounding to bf16
+        ref = R.rotate(x, pos, table, interleaved)
+        amp = R.rotate(x.abs(), pos, table.abs() * torch.tensor(
+            [1.0, -1.0], device=DEV), interleaved).abs() + x.abs().to(F64)
+        err = BF16_HALF * ref.abs() + 2.0 ** -22 * amp
+        assert ((got.to(F64) - ref).abs() <= err).all()
+
+    if heads:
+        near(q_out, q)
+    keep = slots >= 0
+    at = slots[keep].long()
+    flat_k, flat_v = kc.flatten(0, 1), vc.flatten(0, 1)
+    full = torch.zeros(tokens, kv, dim, dtype=BF16, device=DEV)
+    full[keep] = flat_k[at]
+    ref_k = R.rotate(k, pos, table, interleaved)
+    amp = 2 * k.abs().to(F64).amax(-1, keepdim=True)
+    err = (BF16_HALF * ref_k.abs() + 2.0 ** -22 * amp)[keep]
+    assert ((full[keep].to(F64) - ref_k[keep]).abs() <= err).all()
+    assert torch.equal(flat_v[at], v[keep])
+    # every other row of the caches is as it was
+    rest = torch.ones(pages * page, dtype=torch.bool, device=DEV)
+    rest[at] = False
+    assert torch.equal(flat_k[rest], kc0.flatten(0, 1)[rest])
+    assert torch.equal(flat_v[rest], vc0.flatten(0, 1)[rest])
+    assert ops.device_status() == 0
+
+
+def test_paged_append_in_place_without_rotation_and_head_major_cache():
+    g = gen(3)
+    q = randn(g, 6, 2, 64, dt=BF16)
+    k, v = randn(g, 6, 2, 64, dt=BF16), randn(g, 6, 2, 64, dt=BF16)
+    slots = torch.arange(6, dtype=torch.int32, device=DEV) * 3
+    # pages laid out head by head, and one key cache row wider than its values
+    kc = torch.zeros(3, 2, 8, 80, dtype=BF16, device=DEV)[..., :64].transpose(1, 2)
+    vc = torch.zeros(3, 2, 8, 64, dtype=BF16, device=DEV).transpose(1, 2)
+    q0 = q.clone()
+    ops.paged_append(q, k, v, slots, kc, vc, q_out=q)
+    assert torch.equal(q, q0)
+    idx = slots.long()
+    assert torch.equal(kc[idx // 8, idx % 8], k)
+    assert torch.equal(vc[idx // 8, idx % 8], v)
+    pos = torch.arange(6, dtype=torch.int32, device=DEV)
+    ops.paged_append(q, k, v, slots, kc, vc, q_out=q, positions=pos,
+                     rope_cs=rope(8, 64))
+    ref = R.rotate(q0, pos, rope(8, 64), False)
+    assert ((q.to(F64) - ref).abs() <= BF16_HALF * ref.abs() + 2.0 ** -20 *
+            q0.abs().amax()).all()
+
+
+def test_paged_append_rows_outside_the_cache_or_the_table():
+    """Nothing is written for them, and the status word says so once."""
+    g = gen(4)
+    k, v = randn(g, 4, 1, 64, dt=BF16), randn(g, 4, 1, 64, dt=BF16)
+    q = randn(g, 4, 2, 64, dt=BF16)
+    kc = torch.zeros(2, 4, 1, 64, dtype=BF16, device=DEV)
+    vc = torch.zeros_like(kc)
+    q_out = torch.full_like(q, 3.0)
+    slots = torch.tensor([0, 8, 2, -1], dtype=torch.int32, device=DEV)
+    pos = torch.tensor([1, 1, 16, -1], dtype=torch.int32, device=DEV)
+    ops.paged_append(q, k, v, slots, kc, vc, q_out=q_out, positions=pos,
+                     rope_cs=rope(16, 64))
+    assert ops.device_status(reset=True) == _lib.FVB_ERR_INVALID_ARG
+    flat = vc.flatten(0, 1)
+    assert torch.equal(flat[0], v[0]) and (flat[1:] == 0).all()
+    assert (q_out[1:] == 3).all() and not (q_out[0] == 3).any()
+    # padding alone is no error
+    ops.paged_append(q[3:], k[3:], v[3:], slots[3:], kc, vc, q_out=q_out[3:],
+                     positions=pos[3:], rope_cs=rope(16, 64))
+    assert ops.device_status() == 0 and (q_out[3] == 3).all()
+
+
+# --------------------------------------------------------- paged_attention
+def workspace(heads, kv, dim):
+    n = ops.paged_attention_workspace_bytes(heads, kv, dim)
+    return torch.zeros(n, dtype=torch.uint8, device=DEV)
+
+
+def paged_inputs(g, lens, heads, kv, dim, page, head_major=False, width=None):
+    """A cache whose unused rows and table entries would be noticed."""
+    need = [-(-n // page) for n in lens]
+    total = sum(need) + 2
+    width = width or max(need + [1])
+    perm = torch.randperm(total, generator=g, device=DEV).to(torch.int32)
+    table = torch.full((len(lens), width), -7, dtype=torch.int32, device=DEV)
+    shape = (total, kv, page, dim) if head_major else (total, page, kv, dim)
+    kc = torch.full(shape, math.nan, dtype=BF16, device=DEV)
+    vc = torch.full(shape, math.nan, dtype=BF16, device=DEV)
+    if head_major:
+        kc, vc = kc.transpose(1, 2), vc.transpose(1, 2)
+    at = 0
+    for b, n in enumerate(lens):
+        pages = perm[at:at + need[b]]
+        at += need[b]
+        table[b, :need[b]] = pages
+        for c in (kc, vc):
+            rows = torch.full((need[b] * page, kv, dim), math.nan, dtype=BF16,
+                              device=DEV)
+            rows[:n] = randn(g, n, kv, dim, dt=BF16)
+            c[pages.long()] = rows.view(need[b], page, kv, dim)
+    q = randn(g, len(lens), heads, dim, dt=BF16)
+    return q, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+
+def check_attention(out, lse, q, kc, vc, table, lens, scale):
+    """Scores: dim products and sums in f32 (2^-23 each of the magnitudes);
+    a weight is off by that and by 2^-15 (exp2, two bf16 halves, the running
+    rescales); the output by the weights' error, twice for the quotient, and
+    its own rounding."""
+    ref, ref_lse, mag, qk = R.attention(q, kc, vc, table, lens, scale)
+    es = qk * (q.shape[2] + 4) * 2.0 ** -23
+    err = (2 * es + 2.0 ** -15)[..., None] * mag * 2
+    err = err + BF16_HALF * (ref.abs() + err)
+    assert ((out.to(F64) - ref).abs() <= err).all()
+    empty = lens <= 0
+    assert (out[empty] == 0).all() and (lse[empty] == -math.inf).all()
+    d = (lse.to(F64) - ref_lse)[~empty].abs()
+    assert (d <= es[~empty] + 2.0 ** -15 + 2.0 ** -23 * ref_lse[~empty].abs()).all()
+
+
+@pytest.mark.parametrize('heads,kv,dim,page', [
+    (8, 1, 256, 16), (8, 1, 256, 48), (1, 1, 64, 1), (4, 4, 128, 8),
+    (12, 4, 64, 100), (32, 2, 128, 64), (40, 1, 256, 7), (5, 1, 256, 256),
+    (16, 1, 256, 32), (18, 2, 64, 16)])
+def test_paged_attention(heads, kv, dim, page):
+    g = gen(heads * 1000 + dim + page)
+    lens = [0, 1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 0, 300, 867, 5]
+    args = paged_inputs(g, lens, heads, kv, dim, page, head_major=kv > 1)
+    ws = workspace(heads, kv, dim)
+    out = torch.empty_like(args[0])
+    lse = torch.empty(len(lens), heads, device=DEV)
+    for _ in range(2):
+        out.fill_(7.0)
+        lse.fill_(7.0)
+        ops.paged_attention(*args, out, scale=dim ** -0.5, lse=lse,
+                            workspace=ws)
+        check_attention(out, lse, *args, dim ** -0.5)
+        assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize('lens', [
+    [1], [64], [65], [816], [9000], [40000], [0, 0, 0], [0, 20000, 0],
+    [1] * 400, [3000 + 17 * i for i in range(9)],
+    [100000 // (i + 1) for i in range(40)]])
+def test_paged_attention_lengths(lens):
+    """One short sequence, one that every CTA shares, many that share a CTA,
+    and lengths that differ by orders of magnitude."""
+    g = gen(len(lens) + lens[0])
+    args = paged_inputs(g, lens, 8, 1, 128, 64)
+    ws = workspace(8, 1, 128)
+    out = torch.empty_like(args[0])
+    lse = torch.empty(len(lens), 8, device=DEV)
+    ops.paged_attention(*args, out, scale=0.2, lse=lse, workspace=ws)
+    check_attention(out, lse, *args, 0.2)
+    again, lse2 = torch.empty_like(out), torch.empty_like(lse)
+    ops.paged_attention(*args, again, scale=0.2, lse=lse2, workspace=ws)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+def test_paged_attention_views_large_scores_and_no_lse():
+    g = gen(11)
+    lens = [130, 7, 1000]
+    q, kc, vc, table, ln = paged_inputs(g, lens, 4, 2, 64, 16, width=90)
+    wide = randn(g, 3, 4 * 64 + 6, dt=BF16)
+    q = wide[:, 2:258].unflatten(1, (4, 64))
+    outw = torch.full((3, 8, 64), 9.0, dtype=BF16, device=DEV)
+    out = outw[:, 2:6]
+    scale = 30.0       # weights of 0 and 1 nearly everywhere
+    ws = workspace(4, 2, 64)
+    ops.paged_attention(q, kc, vc, table[:, :70], ln, out, scale=scale,
+                        workspace=ws)
+    lse = torch.empty(3, 4, device=DEV)
+    out2 = torch.empty(3, 4, 64, dtype=BF16, device=DEV)
+    ops.paged_attention(q, kc, vc, table, ln, out2, scale=scale, lse=lse,
+                        workspace=ws)
+    assert torch.equal(out, out2)
+    check_attention(out2, lse, q, kc, vc, table, ln, scale)
+    assert (outw[:, :2] == 9).all() and (outw[:, 6:] == 9).all()
+
+
+def test_paged_attention_bad_lengths_and_pages_are_reported():
+    g = gen(12)
+    q, kc, vc, table, ln = paged_inputs(g, [20, 33, 40], 2, 1, 64, 16)
+    kc.nan_to_num_(0.5)
+    vc.nan_to_num_(0.5)
+    ws = workspace(2, 1, 64)
+    out = torch.empty_like(q)
+    lse = torch.empty(3, 2, device=DEV)
+    good = torch.empty_like(q)
+    ops.paged_attention(q, kc, vc, table, ln, good, scale=0.1, workspace=ws)
+    bad_len = ln.clone()
+    bad_len[0], bad_len[2] = -3, 1000     # taken as 0 and as 48 keys
+    ops.paged_attention(q, kc, vc, table, bad_len, out, scale=0.1, lse=lse,
+                        workspace=ws)
+    assert ops.device_status(reset=True) == _lib.FVB_ERR_INVALID_ARG
+    assert (out[0] == 0).all() and torch.equal(out[1], good[1])
+    bad = table.clone()
+    bad[1, 1] = kc.shape[0]
+    ops.paged_attention(q, kc, vc, bad, ln, out, scale=0.1, workspace=ws)
+    assert ops.device_status(reset=True) == _lib.FVB_ERR_INVALID_ARG
+    assert torch.equal(out[0], good[0]) and torch.equal(out[2], good[2])
+    ops.paged_attention(q, kc, vc, table, ln, out, scale=0.1, workspace=ws)
+    assert ops.device_status() == 0 and torch.equal(out, good)
+
+
+def test_paged_attention_offsets_beyond_32_bits():
+    """Pages more than 2^32 bytes and 2^31 elements apart."""
+    g = gen(13)
+    page, dim = 16, 64
+    step = (1 << 30) + 16 * dim * 2                 # elements between pages
+    pool = torch.empty(2 * step + page * dim, dtype=BF16, device=DEV)
+    kc = pool.as_strided((3, page, 1, dim), (step, dim, dim, 1))
+    vc = torch.empty(3, page, 1, dim, dtype=BF16, device=DEV)
+    k, v = randn(g, 48, 1, dim, dt=BF16), randn(g, 48, 1, dim, dt=BF16)
+    slots = torch.arange(48, dtype=torch.int32, device=DEV)
+    ops.paged_append(None, k, v, slots, kc, vc)
+    assert torch.equal(kc.reshape(48, 1, dim), k)
+    q = randn(g, 1, 4, dim, dt=BF16)
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device=DEV)
+    ln = torch.tensor([45], dtype=torch.int32, device=DEV)
+    out = torch.empty_like(q)
+    lse = torch.empty(1, 4, device=DEV)
+    ops.paged_attention(q, kc, vc, table, ln, out, scale=0.125, lse=lse,
+                        workspace=workspace(4, 1, dim))
+    check_attention(out, lse, q, kc, vc, table, ln, 0.125)
+
+
+def test_shapes_that_share_a_workspace_and_captured_calls():
+    """One workspace over several shapes; a captured append + attention whose
+    lengths grow between replays; another stream."""
+    g = gen(14)
+    ws = torch.zeros(max(ops.paged_attention_workspace_bytes(40, 1, 256),
+                         ops.paged_attention_workspace_bytes(8, 1, 64)),
+                     dtype=torch.uint8, device=DEV)
+    for lens, heads, kv, dim in (([5000, 3], 40, 1, 256), ([700] * 90, 8, 1, 64),
+                                 ([5000, 3], 8, 2, 128)):
+        args = paged_inputs(g, lens, heads, kv, dim, 32)
+        out = torch.empty_like(args[0])
+        lse = torch.empty(len(lens), heads, device=DEV)
+        ops.paged_attention(*args, out, scale=0.1, lse=lse, workspace=ws)
+        check_attention(out, lse, *args, 0.1)
+
+    lens = [100, 63, 2000]
+    q, kc, vc, table, ln = paged_inputs(g, [n + 40 for n in lens], 8, 1, 256, 16)
+    kc.nan_to_num_(0.25)
+    vc.nan_to_num_(0.25)
+    ln.copy_(torch.tensor(lens, device=DEV))
+    x = randn(g, 3, 10, 256, dt=BF16)
+    rows = torch.arange(3, device=DEV)
+    slots = torch.empty(3, dtype=torch.int32, device=DEV)
+    pos = torch.empty(3, dtype=torch.int32, device=DEV)
+    cs = rope(4096, 256)
+    out = torch.empty_like(q)
+    lse = torch.empty(3, 8, device=DEV)
+
+    def step():
+        ops.paged_append(x[:, :8], x[:, 8:9], x[:, 9:], slots, kc, vc, q_out=q,
+                         positions=pos, rope_cs=cs)
+        ops.paged_attention(q, kc, vc, table, ln, out, scale=0.0625, lse=lse,
+                            workspace=ws)
+
+    def place(at):
+        pos.copy_(at)
+        ln.copy_(at + 1)
+        page = table[rows, (at // 16).long()]
+        slots.copy_(page * 16 + at % 16)
+
+    at = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    place(at)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        step()
+        side.synchronize()
+        check_attention(out, lse, q, kc, vc, table, ln, 0.0625)
+        with torch.cuda.graph(graph, stream=side):
+            step()
+    for i in range(30):
+        at += 1
+        place(at)
+        x.copy_(randn(g, 3, 10, 256, dt=BF16))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(out, lse, q, kc, vc, table, ln, 0.0625)
+        assert torch.equal(vc[table[rows, (at // 16).long()].long(), (at % 16).long()],
+                           x[:, 9:])
+    assert ops.device_status() == 0
+
+
+# ------------------------------------------------------- the run of them all
+@pytest.mark.parametrize('tokens', [1, 5, 70])
+def test_decoder_layer_of_one_token_per_request(tokens):
+    """norm -> qkv -> append -> attention -> codes -> o -> residual + norm ->
+    gate/up -> codes -> down, each step against its formula on what the step
+    before it gave."""
+    g = gen(20 + tokens)
+    width, heads, dim, mlp, page = 512, 4, 128, 1024, 16
+    qkv_w, qkv_s = pack.quantize_blocks(randn(g, (heads + 2) * dim, width) * 0.05)
+    o_w, o_s = pack.quantize_blocks(randn(g, width, heads * dim) * 0.05)
+    gu_w, gu_s = pack.quantize_blocks(pack.pack_geglu(
+        randn(g, mlp, width) * 0.05, randn(g, mlp, width) * 0.05))
+    dn_w, dn_s = pack.quantize_blocks(randn(g, width, mlp) * 0.05)
+    w1, w2 = randn(g, width, dt=BF16) * 0.1, randn(g, width, dt=BF16) * 0.1
+    lens = [(37 * i) % 200 + 1 for i in range(tokens)]      # new token included
+    _, kc, vc, table, ln = paged_inputs(g, lens, heads, 1, dim, page)
+    at = ln - 1
+    rows = torch.arange(tokens, device=DEV)
+    slots = (table[rows, (at // page).long()] * page + at % page).to(torch.int32)
+    cs = rope(256, dim)
+    x = randn(g, tokens, width)
+    ws = workspace(heads, 1, dim)
+
+    def codes(mode, x, **kw):
+        q = torch.empty(x.shape, dtype=E4M3, device=DEV)
+        s = torch.empty(x.shape[0], -(-x.shape[1] // 128), device=DEV)
+        res = torch.empty_like(x) if 'delta' in kw else None
+        ops.norm_fp8(MODES[mode], x, q, s, res=res, **kw)
+        check_norm(mode, x, kw, q, s, res)
+        return q, s, res
+
+    def product(a, sa, b, sb, epi='bf16'):
+        n = b.shape[0] // 2 if epi == 'geglu' else b.shape[0]
+        out = torch.empty(tokens, n, dtype=F32 if epi == 'f32' else BF16, device=DEV)
+        ops.gemm_fp8(a, sa, b, sb, out, epilogue=EPIS[epi])
+        check_gemm(out, a, sa, b, sb, EPIS[epi])
+        return out
+
+    a, sa, _ = codes('gemma', x, w=w1)
+    qkv = product(a, sa, qkv_w, qkv_s).unflatten(1, (heads + 2, dim))
+    q = torch.empty(tokens, heads, dim, dtype=BF16, device=DEV)
+    ops.paged_append(qkv[:, :heads], qkv[:, heads:heads + 1], qkv[:, heads + 1:],
+                     slots, kc, vc, q_out=q, positions=at, rope_cs=cs)
+    ref = R.rotate(qkv[:, :heads], at, cs, False)
+    assert ((q.to(F64) - ref).abs() <= BF16_HALF * ref.abs() + 2.0 ** -20 *
+            qkv.abs().amax()).all()
+    o = torch.empty_like(q)
+    lse = torch.empty(tokens, heads, device=DEV)
+    ops.paged_attention(q, kc, vc, table, ln, o, scale=dim ** -0.5, lse=lse,
+                        workspace=ws)
+    check_attention(o, lse, q, kc, vc, table, ln, dim ** -0.5)
+    a, sa, _ = codes('none', o.flatten(1))
+    a, sa, x2 = codes('gemma', x, w=w2, delta=product(a, sa, o_w, o_s))
+    h = product(a, sa, gu_w, gu_s, 'geglu')
+    a, sa, _ = codes('none', h)
+    y = x2 + product(a, sa, dn_w, dn_s, 'f32')
+    assert torch.isfinite(y).all() and ops.device_status() == 0
