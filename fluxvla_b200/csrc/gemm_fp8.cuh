@@ -2,23 +2,35 @@
 //   C[t, f] = sum_g sa[t, g] * sb[f / 128, g] * (sum_{k in group g} a[t,k] b[f,k])
 // with one f32 scale per 128 columns of a token row and one per 128 x 128
 // block of the weights.  The scales differ from group to group, so each
-// group's product (128 columns, four MMAs of K = 32) goes to its own
-// accumulator in TMEM and is scaled into f32 registers while the next
-// group's product runs into the other accumulator.
+// group's product (128 columns, four MMAs of K = 32) goes to an accumulator of
+// its own in TMEM and is scaled into f32 registers while the next groups'
+// products run into the others.
 //
-//   warp 0     TMA producer: ring of (A, B) tiles of 128 bytes a row
-//   warp 1     tcgen05.mma issuer, two TMEM accumulators of BN columns
-//   warps 2..  read TMEM (warp w: lanes 32*(w%4)..+31), multiply by the
-//              group's scales, accumulate
+// TMEM lanes are the M side, and a warp reads 32 of them.  With token rows on
+// the M side a lane's factor sa * sb is one register for all its columns.
+// With the features there (SWAP: up to 64 tokens, which would leave half or
+// more of 128 rows empty) the factor varies along the columns and comes from
+// shared memory, 4 bytes for each product; that read costs 128 * BN * 4 bytes
+// of shared-memory bandwidth a group, 256 clocks at 64 tokens, less than the
+// group's weights take from HBM, but twice the MMA's own time at 128.
 //
-// Orientation: the M side (TMEM lanes) holds 128 token rows and the N side BN
-// features; with SWAP (few tokens) the M side holds 128 features, so that the
-// weights fill the 128 rows of the tensor core, and the N side BN tokens.
+//   warp 0      TMA producer: ring of (A, B) tiles of 128-byte rows
+//   warp 1      tcgen05.mma issuer
+//   warp 2      SWAP: column factors, four groups at a time, two batches ahead
+//   warps 4..11 read TMEM (warp w: lanes 32*(w%4)..+31, half of the columns),
+//               multiply by the factors, accumulate
 //
-// CL CTAs of a cluster share a tile, each with a part of the groups; their f32
-// partial tiles are summed through distributed shared memory in the order of
-// the groups, so a product is the same from call to call and needs no
-// workspace.
+// Two kernels:
+//   gemm_fp8_cluster  one tile per CTA (128 tokens x 64 features, or 128
+//                     features x 16, 32 or 64 tokens), the groups split over
+//                     the CTAs of a cluster: enough CTAs to fill the GPU
+//                     however few the tiles are.  The partial tiles are
+//                     exchanged through distributed shared memory and summed
+//                     in the order of the groups, so a product is the same
+//                     from call to call and needs no workspace.
+//   gemm_fp8_pair     256 tokens x 256 features on two SMs (cta_group::2, each
+//                     SM loads half of the features), persistent: for many
+//                     tiles.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -29,32 +41,55 @@ namespace fvb {
 namespace g8 {
 
 constexpr int GROUP = 128;
+constexpr int BATCH = 4;  // groups of one batch of column factors
+constexpr int THREADS = 384;
+constexpr int SCALE_WARP = 2, FIRST_SUM_WARP = 4;
 
 struct Dev {
-  int m, n, k;       // tokens, features, columns
+  int m, n;          // tokens, features
   int groups;        // of 128 columns
-  int m_tiles;       // tiles along the M side
-  int cl;            // CTAs of a cluster
+  int f_tiles;       // feature tiles
+  int t_tiles;       // token tiles
+  int cl_log2;       // CTAs of a cluster (gemm_fp8_cluster)
   const float* sa;   // [tokens, groups]
   long long ld_sa;
   const float* sb;   // [features / 128, groups]
   long long ld_sb;
   void* out;
   long long ldo;
-  int vec_out;       // rows of out take 16-byte (bf16: 8-byte) stores
+  int vec_out;       // rows of out take 16-byte stores
 };
 
 // kind::f8f6f4, e4m3 x e4m3 -> f32, both K-major
 __host__ __device__ constexpr uint32_t idesc_e4m3_f32(int M, int N) {
   return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
+template <int CTAS>
 __device__ __forceinline__ void mma_e4m3(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
                                          uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+  if (CTAS == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+
+// true in one lane of a converged warp.  The issuing warps run their loops
+// with all lanes and only the MMAs and commits in this one: addresses and
+// descriptors then stay warp-uniform (a loop of one lane measured 0.05 us more
+// per group of the pair kernel).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(r));
+  return r != 0;
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -62,82 +97,254 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 }
-__device__ __forceinline__ float4 ld_cluster4(uint32_t saddr, uint32_t rank) {
-  uint32_t a;
-  float4 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(a)
-               : "memory");
-  return v;
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t mapa(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
 }
 
-// gelu(x) with the tanh form, as x / (1 + exp(-2u)): no cancellation where
-// the tanh nears -1
-__device__ __forceinline__ float gelu_sigmoid(float x) {
-  const float u2 = 1.5957691216057308f * (x + 0.044715f * x * x * x);
-  return x / (1.f + __expf(-u2));
+// 32 TMEM lanes x N columns into registers; tmem_wait makes them valid
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* r);
+template <>
+__device__ __forceinline__ void tmem_ld<8>(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                 "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+template <>
+__device__ __forceinline__ void tmem_ld<16>(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+template <>
+__device__ __forceinline__ void tmem_ld<32>(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(taddr));
+}
+template <int N>
+__device__ __forceinline__ void tmem_wait(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  // the registers are read only after the wait
+#pragma unroll
+  for (int j = 0; j < N; ++j) asm volatile("" : "+r"(r[j]));
 }
 
+// acc[N] += r[N] * cs[N] (cs: 16-byte aligned shared memory, read by all lanes)
+template <int N>
+__device__ __forceinline__ void scale_add(float* acc, const uint32_t* r, const float* cs) {
+#pragma unroll
+  for (int j = 0; j < N; j += 4) {
+    const float4 s = *reinterpret_cast<const float4*>(cs + j);
+    acc[j] = fmaf(__uint_as_float(r[j]), s.x, acc[j]);
+    acc[j + 1] = fmaf(__uint_as_float(r[j + 1]), s.y, acc[j + 1]);
+    acc[j + 2] = fmaf(__uint_as_float(r[j + 2]), s.z, acc[j + 2]);
+    acc[j + 3] = fmaf(__uint_as_float(r[j + 3]), s.w, acc[j + 3]);
+  }
+}
+// acc[N] += r[N] * f
+template <int N>
+__device__ __forceinline__ void scale_add(float* acc, const uint32_t* r, float f) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) acc[j] = fmaf(__uint_as_float(r[j]), f, acc[j]);
+}
+
+// gelu(x) * up for two pairs, gelu in its tanh form as x / (1 + exp(-2u)): no
+// cancellation where the tanh nears -1.  One reciprocal serves both; the
+// exponents are capped at 2^60 so that the product of the two stays finite.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void geglu2(float x0, float u0, float x1, float u1, float& y0,
+                                       float& y1) {
+  constexpr float C1 = -2.3022081985f, C3 = C1 * 0.044715f;  // -2 sqrt(2/pi) log2(e)
+  const float d0 = 1.f + ex2(fminf(x0 * fmaf(C3, x0 * x0, C1), 60.f));
+  const float d1 = 1.f + ex2(fminf(x1 * fmaf(C3, x1 * x1, C1), 60.f));
+  const float r = __fdividef(1.f, d0 * d1);
+  y0 = x0 * u0 * (r * d1);
+  y1 = x1 * u1 * (r * d0);
+}
+
+// Writes NF consecutive features f.. of token t (NF = 4, 8 or 16; for GEGLU
+// features 2i, 2i+1 are gate and up of output i), cut at the last feature.
+template <int NF, int EPI>
+__device__ __forceinline__ void store_features(const Dev& p, int t, int f, const float (&v)[NF]) {
+  if (t >= p.m || f >= p.n) return;
+  const int nf = min(NF, p.n - f);
+  if (EPI == FVB_EPI_F32_STORE) {
+    float* o = static_cast<float*>(p.out) + (long long)t * p.ldo + f;
+    if (p.vec_out && nf == NF) {
+#pragma unroll
+      for (int j = 0; j < NF; j += 4)
+        *reinterpret_cast<float4*>(o + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NF; ++j)
+        if (j < nf) o[j] = v[j];
+    }
+    return;
+  }
+  constexpr int NO = EPI == FVB_EPI_GEGLU ? NF / 2 : NF;
+  const int no = EPI == FVB_EPI_GEGLU ? nf / 2 : nf;
+  float y[NO];
+#pragma unroll
+  for (int j = 0; j < NO; j += 2) {
+    if (EPI == FVB_EPI_GEGLU) {
+      geglu2(v[2 * j % NF], v[(2 * j + 1) % NF], v[(2 * j + 2) % NF], v[(2 * j + 3) % NF], y[j],
+             y[j + 1]);
+    } else {
+      y[j] = v[j];
+      y[j + 1] = v[j + 1];
+    }
+  }
+  bf16* o = static_cast<bf16*>(p.out) + (long long)t * p.ldo + (EPI == FVB_EPI_GEGLU ? f >> 1 : f);
+  if (p.vec_out && no == NO) {
+    uint32_t w[NO / 2];
+#pragma unroll
+    for (int j = 0; j < NO; j += 2) w[j / 2] = pack_bf16x2(y[j], y[j + 1]);
+    if (NO == 8)
+      *reinterpret_cast<uint4*>(o) =
+          make_uint4(w[0], w[1 % (NO / 2)], w[2 % (NO / 2)], w[3 % (NO / 2)]);
+    else if (NO == 4)
+      *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1 % (NO / 2)]);
+    else
+      *reinterpret_cast<uint32_t*>(o) = w[0];
+  } else {
+#pragma unroll
+    for (int j = 0; j < NO; ++j)
+      if (j < no) o[j] = __float2bfloat16(y[j]);
+  }
+}
+
+// The factor warp: sa * sb of token rows t0..t0+ROWS-1 and BLOCKS feature
+// blocks for the groups g0..g1, a batch of four groups at a time into
+// fac[slot][block][row][group] (or [slot][group][row], COLUMNS).  Lanes run
+// over the groups first: 16 bytes of a row are one access, where a load of
+// one group for 32 rows would touch 32 lines, and every summing warp would
+// repeat it.  bt counts batches over a CTA's tiles.
+template <int ROWS, int BLOCKS, bool COLUMNS>
+__device__ __forceinline__ bool write_factors(const Dev& p, int t0, int block, int g0, int g1,
+                                              float* fac, uint64_t* ffull, uint64_t* fempty,
+                                              int& bt, int lane) {
+  static_assert(!COLUMNS || BLOCKS == 1, "layout");
+  const int e = lane & (BATCH - 1), r0 = lane / BATCH;
+  const int last = (p.n - 1) / 128;
+  for (int g = g0; g < g1; g += BATCH, ++bt) {
+    const int ge = min(g + e, g1 - 1), slot = bt & 1;
+    float a[ROWS / 8], b[BLOCKS];
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i)
+      b[i] = __ldg(p.sb + (long long)min(block + i, last) * p.ld_sb + ge);
+#pragma unroll
+    for (int i = 0; i < ROWS / 8; ++i)
+      a[i] = __ldg(p.sa + (long long)min(t0 + i * 8 + r0, p.m - 1) * p.ld_sa + ge);
+    if (!mbar_wait(&fempty[slot], ((bt >> 1) & 1) ^ 1)) return false;
+    float* f = fac + slot * (BATCH * ROWS * BLOCKS);
+#pragma unroll
+    for (int i = 0; i < ROWS / 8; ++i) {
+      const int row = i * 8 + r0;
+      if (COLUMNS) {
+        f[e * ROWS + row] = a[i] * b[0];
+      } else {
+#pragma unroll
+        for (int j = 0; j < BLOCKS; ++j) f[(j * ROWS + row) * BATCH + e] = a[i] * b[j];
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ffull[slot]);
+  }
+  return true;
+}
+__device__ __forceinline__ float pick(const float4& v, int e) {
+  return e == 0 ? v.x : (e == 1 ? v.y : (e == 2 ? v.z : v.w));
+}
+
+// ---------------------------------------------------------------------------
+// one tile per CTA, groups split over a cluster
+// ---------------------------------------------------------------------------
 template <int BN, bool SWAP>
 struct Cfg {
+  static_assert(BN <= 64, "two CTAs share an SM's TMEM and registers");
   static constexpr int A_BYTES = 128 * GROUP;
-  static constexpr int B_BYTES = BN * GROUP;
-  static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = (196 * 1024) / STAGE < 8 ? (196 * 1024) / STAGE : 8;
-  static constexpr int PW = SWAP ? 4 : 8;            // scaling warps
-  static constexpr int COLS = SWAP ? BN : BN / 2;    // accumulator columns of a warp
-  static constexpr int THREADS = 64 + 32 * PW;
-  // finished tile in shared memory: [tokens][features + 4] f32, over the ring
-  static constexpr int T_ROWS = SWAP ? BN : 128;
-  static constexpr int T_COLS = SWAP ? 128 : BN;
-  static constexpr int PITCH = T_COLS + 4;
-  static_assert(T_ROWS * PITCH * 4 <= STAGES * STAGE, "the finished tile reuses the ring");
-  static constexpr int OFF_CS = STAGES * STAGE;      // SWAP: [PW][2][BN] column scales
-  static constexpr int OFF_BAR = OFF_CS + (SWAP ? PW * 2 * BN * 4 : 0);
-  static constexpr int SMEM = OFF_BAR + (2 * STAGES + 4) * 8 + 16 + 1024;
-  static constexpr uint32_t TMEM_COLS =
-      2 * BN <= 32 ? 32 : (2 * BN <= 64 ? 64 : (2 * BN <= 128 ? 128 : (2 * BN <= 256 ? 256 : 512)));
+  static constexpr int STAGE = A_BYTES + BN * GROUP;
+  static constexpr int STAGES = BN == 16 ? 5 : (BN == 32 ? 4 : 3);
+  static constexpr int NB = 4;                       // accumulators
+  static constexpr int COLS = BN / 2;                // columns of a warp
+  static constexpr uint32_t TMEM_COLS = NB * BN;
+  // partials [tokens][features] f32; rows written lane by lane are padded
+  static constexpr int T_ROWS = SWAP ? BN : 128, F_COLS = SWAP ? 128 : BN;
+  static constexpr int PITCH = SWAP ? 128 : BN + 4;
+  static constexpr int OFF_RECV = STAGES * STAGE;
+  static constexpr int OFF_CS = OFF_RECV + T_ROWS * PITCH * 4;
+  static constexpr int OFF_BAR = OFF_CS + 2 * BATCH * T_ROWS * 4;
+  static constexpr int SMEM = OFF_BAR + (2 * STAGES + 2 * NB + 4) * 8 + 16 + 1024;
 };
 
 template <int BN, bool SWAP, int EPI>
-__global__ void __launch_bounds__(Cfg<BN, SWAP>::THREADS, 1)
-    gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA,
-                    const __grid_constant__ CUtensorMap tmB, const Dev p) {
+__global__ void __launch_bounds__(THREADS, 2)
+    gemm_fp8_cluster(const __grid_constant__ CUtensorMap tmA,
+                     const __grid_constant__ CUtensorMap tmB, const Dev p) {
   using C = Cfg<BN, SWAP>;
-  constexpr int COLS = C::COLS;
+  constexpr int COLS = C::COLS, NB = C::NB;
+  constexpr int LD = COLS < 32 ? COLS : 32;  // columns of one TMEM read
   constexpr uint32_t IDESC = idesc_e4m3_f32(128, BN);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* cs = reinterpret_cast<float*>(smem + C::OFF_CS);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* empty = full + C::STAGES;
-  uint64_t* tfull = empty + C::STAGES;  // [2]
-  uint64_t* tempty = tfull + 2;         // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint64_t* tfull = empty + C::STAGES;  // [NB]
+  uint64_t* tempty = tfull + NB;        // [NB]
+  uint64_t* csfull = tempty + NB;       // [2]
+  uint64_t* csempty = csfull + 2;       // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(csempty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cl = p.cl;
+  const int cl = 1 << p.cl_log2;
   const uint32_t rank = cl > 1 ? cluster_rank() : 0;
-  const int tile = blockIdx.x / cl;
-  const int mt = tile % p.m_tiles, nt = tile / p.m_tiles;
-  const int g0 = (int)((long long)p.groups * rank / cl);
-  const int g1 = (int)((long long)p.groups * (rank + 1) / cl);
+  const int tile = blockIdx.x >> p.cl_log2;
+  const int ft = tile % p.f_tiles, tt = tile / p.f_tiles;
+  const int f0 = ft * C::F_COLS, t0 = tt * C::T_ROWS;
+  const int g0 = (int)(((long long)p.groups * rank) >> p.cl_log2);
+  const int g1 = (int)(((long long)p.groups * (rank + 1)) >> p.cl_log2);
   const int ng = g1 - g0;
+  const int per = C::T_ROWS >> p.cl_log2;  // token rows that each CTA sums
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < NB; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], C::PW);
+      mbar_init(&tempty[a], 8);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&csfull[a], 1);
+      mbar_init(&csempty[a], 8);
     }
     fence_barrier_init();
     prefetch_tensormap(&tmA);
@@ -147,187 +354,442 @@ __global__ void __launch_bounds__(Cfg<BN, SWAP>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (cl > 1) cluster_arrive();  // waited for before the first remote store
   const uint32_t tmem = *tmem_slot;
-  bool ok = true;
+  griddep_wait();
+  griddep_launch_dependents();
 
   if (warp == 0) {
     if (lane == 0) {
-      const CUtensorMap* mw = SWAP ? &tmA : &tmB;
-      const CUtensorMap* mx = SWAP ? &tmB : &tmA;
-      constexpr int woff = SWAP ? 0 : C::A_BYTES, xoff = SWAP ? C::A_BYTES : 0;
-      const int wrow = SWAP ? mt * 128 : nt * BN, xrow = SWAP ? nt * BN : mt * 128;
-      griddep_wait();
       for (int i = 0; i < ng; ++i) {
         const int s = i % C::STAGES;
-        if (!mbar_wait(&empty[s], ((i / C::STAGES) & 1) ^ 1)) break;
+        if (!mbar_wait_spin(&empty[s], ((i / C::STAGES) & 1) ^ 1)) break;
         mbar_arrive_expect_tx(&full[s], C::STAGE);
-        tma_load_2d(smem + s * C::STAGE + woff, mw, (g0 + i) * GROUP, wrow, &full[s]);
-        tma_load_2d(smem + s * C::STAGE + xoff, mx, (g0 + i) * GROUP, xrow, &full[s]);
+        uint8_t* sa = smem + s * C::STAGE;
+        tma_load_2d(sa, &tmA, (g0 + i) * GROUP, SWAP ? f0 : t0, &full[s]);
+        tma_load_2d(sa + C::A_BYTES, &tmB, (g0 + i) * GROUP, SWAP ? t0 : f0, &full[s]);
       }
-      griddep_launch_dependents();
     }
+    __syncwarp();
+    if (cl > 1) cluster_wait();
   } else if (warp == 1) {
-    if (lane == 0) {
-      for (int i = 0; i < ng; ++i) {
-        const int s = i % C::STAGES, b = i & 1;
-        if (!mbar_wait(&tempty[b], ((i >> 1) & 1) ^ 1)) break;
-        if (!mbar_wait(&full[s], (i / C::STAGES) & 1)) break;
-        tc_fence_after();
+    const bool elected = elect_one();
+    for (int i = 0; i < ng; ++i) {
+      const int s = i % C::STAGES, b = i % NB;
+      bool ready = mbar_wait_spin(&full[s], (i / C::STAGES) & 1);
+      ready = ready && mbar_wait_spin(&tempty[b], ((i / NB) & 1) ^ 1);
+      if (!__all_sync(0xffffffffu, ready)) break;
+      tc_fence_after();
+      if (elected) {
         const uint64_t da = smem_desc_sw128(smem_u32(smem + s * C::STAGE));
         const uint64_t db = smem_desc_sw128(smem_u32(smem + s * C::STAGE + C::A_BYTES));
 #pragma unroll
         for (int kk = 0; kk < GROUP / 32; ++kk)
-          mma_e4m3(tmem + b * BN, da + kk * 2, db + kk * 2, IDESC, kk > 0);
-        tc_commit(&empty[s]);
+          mma_e4m3<1>(tmem + b * BN, da + kk * 2, db + kk * 2, IDESC, kk > 0);
         tc_commit(&tfull[b]);
+        tc_commit(&empty[s]);
       }
+      __syncwarp();
     }
+    if (cl > 1) cluster_wait();
+  } else if (warp < FIRST_SUM_WARP) {
+    int bt = 0;
+    if (warp == SCALE_WARP)
+      write_factors<C::T_ROWS, 1, SWAP>(p, t0, f0 / 128, g0, g1, cs, csfull, csempty, bt, lane);
+    if (cl > 1) cluster_wait();
   } else {
-    const int q = warp & 3, half = SWAP ? 0 : (warp - 2) >> 2;
-    const int row = mt * 128 + q * 32 + lane;  // token (SWAP: feature) of this thread
-    const int col0 = nt * BN + half * COLS;    // first feature (SWAP: token)
-    griddep_wait();
+    const int q = warp & 3, half = (warp - FIRST_SUM_WARP) >> 2;
     float acc[COLS];
 #pragma unroll
     for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
-    // scales are read one group ahead
-    const float* sa_row = p.sa + (long long)min(row, p.m - 1) * p.ld_sa;
-    const int sb_tile = SWAP ? mt : min(col0, p.n - 1) / GROUP;
-    const float* sb_row = p.sb + (long long)sb_tile * p.ld_sb;
-    float* cs = reinterpret_cast<float*>(smem + C::OFF_CS) + (SWAP ? (warp - 2) * 2 * BN : 0);
-    constexpr int CPL = SWAP ? (BN + 31) / 32 : 1;  // column scales of a lane
-    float sa_next[CPL], sb_next = 0.f;
-    auto fetch = [&](int g) {
-      sb_next = __ldg(sb_row + g);
-      if (SWAP) {
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-          const int t = min(col0 + c * 32 + lane, p.m - 1);
-          sa_next[c] = __ldg(p.sa + (long long)t * p.ld_sa + g);
-        }
-      } else {
-        sa_next[0] = __ldg(sa_row + g);
-      }
-    };
-    if (ng > 0) fetch(g0);
     const uint32_t lane_base = tmem + ((uint32_t)(q * 32) << 16) + half * COLS;
-    for (int i = 0; i < ng; ++i) {
-      const int b = i & 1;
-      float scale = sb_next;
-      if (SWAP) {
-#pragma unroll
-        for (int c = 0; c < CPL; ++c)
-          if (c * 32 + lane < BN) cs[b * BN + c * 32 + lane] = sa_next[c] * scale;
+    bool ok = true;
+    for (int i0 = 0; i0 < ng && ok; i0 += BATCH) {
+      const int slot = (i0 / BATCH) & 1;
+      ok = mbar_wait_spin(&csfull[slot], (i0 / (2 * BATCH)) & 1);
+      float4 f4;
+      if (!SWAP) {
+        f4 = reinterpret_cast<const float4*>(cs)[slot * 128 + q * 32 + lane];
         __syncwarp();
-      } else {
-        scale *= sa_next[0];
+        if (lane == 0) mbar_arrive(&csempty[slot]);
       }
-      if (i + 1 < ng) fetch(g0 + i + 1);
-      ok = mbar_wait(&tfull[b], (i >> 1) & 1);
-      __syncwarp();
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      tc_fence_after();
-      const uint32_t ta = lane_base + b * BN;
 #pragma unroll
-      for (int c = 0; c < COLS; c += 16) {
-        uint32_t r[16];
-        tmem_ld16_sync(ta + c, r);
-        if (SWAP) {
+      for (int e = 0; e < BATCH; ++e) {
+        const int i = i0 + e, b = i % NB;
+        if (i < ng && ok) {
+          ok = mbar_wait_spin(&tfull[b], (i / NB) & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok) {
+            tc_fence_after();
+            const uint32_t ta = lane_base + b * BN;
+            uint32_t r[COLS];
 #pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            const float4 s = *reinterpret_cast<const float4*>(cs + b * BN + c + j);
-            acc[c + j] = fmaf(__uint_as_float(r[j]), s.x, acc[c + j]);
-            acc[c + j + 1] = fmaf(__uint_as_float(r[j + 1]), s.y, acc[c + j + 1]);
-            acc[c + j + 2] = fmaf(__uint_as_float(r[j + 2]), s.z, acc[c + j + 2]);
-            acc[c + j + 3] = fmaf(__uint_as_float(r[j + 3]), s.w, acc[c + j + 3]);
+            for (int j = 0; j < COLS; j += LD) tmem_ld<LD>(ta + j, r + j);
+            tmem_wait<COLS>(r);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tempty[b]);
+            if (SWAP)
+              scale_add<COLS>(acc, r, cs + (slot * BATCH + e) * BN + half * COLS);
+            else
+              scale_add<COLS>(acc, r, pick(f4, e));
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            acc[c + j] = fmaf(__uint_as_float(r[j]), scale, acc[c + j]);
         }
       }
-      tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[b]);
+      if (SWAP && lane == 0) mbar_arrive(&csempty[slot]);
     }
-    // every product has been read, so the ring is free for the finished tile
-    float* ts = reinterpret_cast<float*>(smem);
+    // each token row goes to the CTA that sums it
+    if (cl > 1) cluster_wait();
     if (ok) {
+      const uint32_t recv = smem_u32(smem + C::OFF_RECV);
       if (SWAP) {
+        // columns are tokens: 32 lanes hold 32 features of one
 #pragma unroll
-        for (int j = 0; j < COLS; ++j) ts[j * C::PITCH + q * 32 + lane] = acc[j];
+        for (int j = 0; j < COLS; ++j) {
+          const int tok = half * COLS + j;
+          const uint32_t at =
+              recv + ((rank * per + (tok & (per - 1))) * C::PITCH + q * 32 + lane) * 4;
+          if (cl > 1)
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa(at, tok / per)),
+                         "f"(acc[j])
+                         : "memory");
+          else
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(acc[j]) : "memory");
+        }
       } else {
+        const int tok = q * 32 + lane;
+        uint32_t at =
+            recv + ((rank * per + (tok & (per - 1))) * C::PITCH + half * COLS) * 4;
+        if (cl > 1) at = mapa(at, tok / per);
 #pragma unroll
-        for (int j = 0; j < COLS; j += 4)
-          *reinterpret_cast<float4*>(ts + (q * 32 + lane) * C::PITCH + half * COLS + j) =
-              make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+        for (int j = 0; j < COLS; j += 4) {
+          if (cl > 1)
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + j * 4),
+                         "f"(acc[j]), "f"(acc[j + 1]), "f"(acc[j + 2]), "f"(acc[j + 3])
+                         : "memory");
+          else
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + j * 4),
+                         "f"(acc[j]), "f"(acc[j + 1]), "f"(acc[j + 2]), "f"(acc[j + 3])
+                         : "memory");
+        }
       }
     }
   }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  if (cl > 1) {
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }
-  if (cl > 1) cluster_sync();
-
-  // this CTA's share of the tile's token rows: sum over the cluster, epilogue
-  const uint32_t ts = smem_u32(smem);
-  const int t0 = SWAP ? nt * BN : mt * 128, f0 = SWAP ? mt * 128 : nt * BN;
-  const int r0 = C::T_ROWS * rank / cl, r1 = C::T_ROWS * (rank + 1) / cl;
-  constexpr int Q = C::T_COLS / 4;
-  for (int e = threadIdx.x; e < (r1 - r0) * Q; e += C::THREADS) {
-    const int r = r0 + e / Q, c = (e % Q) * 4;
-    const int t = t0 + r, f = f0 + c;
-    if (t >= p.m || f >= p.n) continue;
-    const uint32_t at = ts + (r * C::PITCH + c) * 4;
-    float4 v;
-    if (cl > 1) {
-      v = ld_cluster4(at, 0);
-      for (int i = 1; i < cl; ++i) {
-        const float4 w = ld_cluster4(at, i);
-        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
-      }
-    } else {
-      v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) +
-                                           r * C::PITCH + c);
+  // this CTA's tokens: the cluster's partials in the order of the groups
+  const float* recv = reinterpret_cast<const float*>(smem + C::OFF_RECV);
+#pragma unroll 4
+  for (int e = threadIdx.x; e < per * (C::F_COLS / 4); e += THREADS) {
+    const int r = e / (C::F_COLS / 4), f = e % (C::F_COLS / 4) * 4;
+    float4 v = *reinterpret_cast<const float4*>(recv + r * C::PITCH + f);
+    for (int i = 1; i < cl; ++i) {
+      const float4 w = *reinterpret_cast<const float4*>(recv + (i * per + r) * C::PITCH + f);
+      v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
     }
-    const int nf = min(4, p.n - f);
-    if (EPI == FVB_EPI_F32_STORE) {
-      float* o = static_cast<float*>(p.out) + (long long)t * p.ldo + f;
-      if (p.vec_out && nf == 4) {
-        *reinterpret_cast<float4*>(o) = v;
-      } else {
-        o[0] = v.x;
-        if (nf > 1) o[1] = v.y;
-        if (nf > 2) o[2] = v.z;
-        if (nf > 3) o[3] = v.w;
-      }
-    } else if (EPI == FVB_EPI_BF16) {
-      bf16* o = static_cast<bf16*>(p.out) + (long long)t * p.ldo + f;
-      if (p.vec_out && nf == 4) {
-        *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
-      } else {
-        o[0] = __float2bfloat16(v.x);
-        if (nf > 1) o[1] = __float2bfloat16(v.y);
-        if (nf > 2) o[2] = __float2bfloat16(v.z);
-        if (nf > 3) o[3] = __float2bfloat16(v.w);
-      }
-    } else {  // FVB_EPI_GEGLU: features 2i, 2i+1 are gate and up of output i
-      bf16* o = static_cast<bf16*>(p.out) + (long long)t * p.ldo + (f >> 1);
-      const float y0 = gelu_sigmoid(v.x) * v.y, y1 = gelu_sigmoid(v.z) * v.w;
-      if (p.vec_out && nf == 4) {
-        *reinterpret_cast<uint32_t*>(o) = pack_bf16x2(y0, y1);
-      } else {
-        o[0] = __float2bfloat16(y0);
-        if (nf > 3) o[1] = __float2bfloat16(y1);
+    const float y[4] = {v.x, v.y, v.z, v.w};
+    store_features<4, EPI>(p, t0 + rank * per + r, f0 + f, y);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// two-SM tiles, persistent
+// ---------------------------------------------------------------------------
+struct PairCfg {
+  static constexpr int TILE = 256;                 // tokens and features of a tile
+  static constexpr int HALF = 128 * GROUP;         // bytes of a CTA's half of either
+  static constexpr int STAGE = 2 * HALF;
+  static constexpr int STAGES = 5;
+  static constexpr int SUM_WARPS = 8;
+  static constexpr int COLS = TILE / 2;
+  static constexpr int OFF_STG = STAGES * STAGE;   // [warps][32 rows][64 bytes]
+  static constexpr int STG = 32 * 64;
+  static constexpr int OFF_F = OFF_STG + SUM_WARPS * STG;  // [2][BATCH][2][128] f32
+  static constexpr int OFF_BAR = OFF_F + 2 * BATCH * 2 * 128 * 4;
+  static constexpr int SMEM = OFF_BAR + (2 * STAGES + 8) * 8 + 16 + 1024;
+};
+
+__device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorMap* map, int32_t x,
+                                                 int32_t y, uint32_t bar_cluster) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::"
+      "complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar_cluster)
+      : "memory");
+}
+__device__ __forceinline__ void commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster."
+      "multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"((unsigned short)0x3)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster) {
+  // relaxed: what it orders are TMEM reads, done before by tcgen05.wait::ld; a
+  // cluster-scope release would wait for this thread's global stores as well
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster)
+               : "memory");
+}
+// bounded wait with cluster-scope acquire (arrivals come from the peer too)
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t t0 = 0;
+  for (uint32_t n = 0;; ++n) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((n & 63) == 0) {
+      const uint64_t t = globaltimer_ns();
+      if (!t0) t0 = t;
+      if (t - t0 > FVB_WAIT_LIMIT_NS) {
+        record_device_error(FVB_ERR_DEVICE_TIMEOUT);
+        return false;
       }
     }
   }
-  if (cl > 1) cluster_sync();  // the others may still read this CTA's tile
+}
+
+template <int EPI>
+__global__ void __launch_bounds__(THREADS, 1)
+    gemm_fp8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                  const Dev p) {
+  using C = PairCfg;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* tfull = empty + C::STAGES;  // [2]
+  uint64_t* tempty = tfull + 2;         // [2] (leader: of both CTAs)
+  uint64_t* ffull = tempty + 2;         // [2]
+  uint64_t* fempty = ffull + 2;         // [2]
+  float* fac = reinterpret_cast<float*>(smem + C::OFF_F);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fempty + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  const int n_tiles = p.f_tiles * p.t_tiles;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 2 * C::SUM_WARPS);
+      mbar_init(&ffull[a], 1);
+      mbar_init(&fempty[a], C::SUM_WARPS);
+    }
+    fence_barrier_init();
+    prefetch_tensormap(&tmA);
+    prefetch_tensormap(&tmB);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncwarp();
+  cluster_arrive();  // barriers of both CTAs initialised, TMEM allocated
+  cluster_wait();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  // 384 threads start with 168 registers each; the eight summing warps take
+  // 208 (128 sums and two TMEM reads of 32) and the first four keep 80:
+  // 256 * 208 + 128 * 80 = 63488 <= 384 * 168.  (Sixteen summing warps of 64
+  // columns measured 80 us against 71 us on 816 x 32768 x 2048.)
+  // Token tiles vary fastest: the pairs at work share weight tiles.
+  if (warp < FIRST_SUM_WARP) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 0 && lane == 0) {
+      int it = 0;
+      bool alive = true;
+      for (int w = pair; w < n_tiles && alive; w += n_pairs) {
+        const int trow = (w % p.t_tiles) * C::TILE + (int)rank * 128;
+        const int wrow = (w / p.t_tiles) * C::TILE + (int)rank * 128;
+        for (int g = 0; g < p.groups; ++g, ++it) {
+          const int s = it % C::STAGES;
+          if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1)) { alive = false; break; }
+          const uint32_t fb = mapa(smem_u32(&full[s]), 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * C::STAGE);
+          uint8_t* sa = smem + s * C::STAGE;
+          tma_load_2d_pair(sa, &tmA, g * GROUP, trow, fb);
+          tma_load_2d_pair(sa + C::HALF, &tmB, g * GROUP, wrow, fb);
+        }
+      }
+    } else if (warp == 1 && rank == 0) {
+      const bool elected = elect_one();
+      constexpr uint32_t IDESC = idesc_e4m3_f32(256, C::TILE);
+      const int n_it = p.groups * ((n_tiles - pair + n_pairs - 1) / n_pairs);
+      int s = 0;
+      uint32_t phase = 0;
+#pragma unroll 1
+      for (int it = 0; it < n_it; ++it) {
+        const int b = it & 1;
+        bool ready = mbar_wait_spin(&full[s], phase);
+        ready = ready && mbar_wait_cluster(&tempty[b], ((it >> 1) & 1) ^ 1);
+        if (!__all_sync(0xffffffffu, ready)) break;
+        tc_fence_after();
+        if (elected) {
+          const uint64_t da = smem_desc_sw128(smem_u32(smem + s * C::STAGE));
+          const uint64_t db = smem_desc_sw128(smem_u32(smem + s * C::STAGE + C::HALF));
+#pragma unroll
+          for (int kk = 0; kk < GROUP / 32; ++kk)
+            mma_e4m3<2>(tmem + b * C::TILE, da + kk * 2, db + kk * 2, IDESC, kk > 0);
+          commit_both(&tfull[b]);
+          commit_both(&empty[s]);
+        }
+        __syncwarp();
+        if (++s == C::STAGES) {
+          s = 0;
+          phase ^= 1;
+        }
+      }
+    } else if (warp == SCALE_WARP) {
+      int bt = 0;
+      bool alive = true;
+      for (int w = pair; w < n_tiles && alive; w += n_pairs)
+        alive = write_factors<128, 2, false>(p, (w % p.t_tiles) * C::TILE + (int)rank * 128,
+                                             (w / p.t_tiles) * 2, 0, p.groups, fac, ffull, fempty,
+                                             bt, lane);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int q = warp & 3, part = (warp - FIRST_SUM_WARP) >> 2;
+    const uint32_t lane_base = tmem + ((uint32_t)(q * 32) << 16) + part * C::COLS;
+    const uint32_t te[2] = {mapa(smem_u32(&tempty[0]), 0), mapa(smem_u32(&tempty[1]), 0)};
+    const uint32_t stg = smem_u32(smem + C::OFF_STG) + (warp - FIRST_SUM_WARP) * C::STG;
+    const float4* frow = reinterpret_cast<const float4*>(fac) + part * 128 + q * 32 + lane;
+    int it = 0, bt = 0;
+    bool ok = true;
+    for (int w = pair; w < n_tiles && ok; w += n_pairs) {
+      const int t0 = (w % p.t_tiles) * C::TILE + (int)rank * 128 + q * 32;
+      const int f0 = (w / p.t_tiles) * C::TILE + part * C::COLS;
+      float acc[C::COLS];
+#pragma unroll
+      for (int j = 0; j < C::COLS; ++j) acc[j] = 0.f;
+      float4 f4;
+#pragma unroll 1
+      for (int g = 0; g < p.groups; ++g, ++it) {
+        const int b = it & 1, e = g & (BATCH - 1), slot = bt & 1;
+        if (e == 0) {
+          ok = mbar_wait_spin(&ffull[slot], (bt >> 1) & 1);
+          f4 = frow[slot * 256];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&fempty[slot]);
+          ++bt;
+        }
+        const float f = pick(f4, e);
+        ok = ok && mbar_wait_spin(&tfull[b], (it >> 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t ta = lane_base + b * C::TILE;
+        uint32_t r[2][32];
+        tmem_ld<32>(ta, r[0]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          tmem_wait<32>(r[j & 1]);
+          if (j < 3) {
+            tmem_ld<32>(ta + 32 * j + 32, r[(j + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(te[b]);
+          }
+          scale_add<32>(acc + 32 * j, r[j & 1], f);
+        }
+      }
+      if (!ok) break;
+      // A lane holds one token's features: 64 bytes of output a row at a time
+      // go through shared memory (16-byte pieces swizzled by the row), so that
+      // each store instruction writes 64 bytes of 8 rows.
+      constexpr int FC = EPI == FVB_EPI_F32_STORE ? 16 : (EPI == FVB_EPI_BF16 ? 32 : 64);
+      const int eb = EPI == FVB_EPI_F32_STORE ? 4 : 2;
+      const int nf_out = EPI == FVB_EPI_GEGLU ? p.n / 2 : p.n;
+#pragma unroll
+      for (int c = 0; c < C::COLS; c += FC) {
+        uint32_t v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (EPI == FVB_EPI_F32_STORE) {
+            v[j] = __float_as_uint(acc[c + j]);
+          } else if (EPI == FVB_EPI_BF16) {
+            v[j] = pack_bf16x2(acc[c + 2 * j], acc[c + 2 * j + 1]);
+          } else {
+            const float* a = acc + c + 4 * j;
+            float y0, y1;
+            geglu2(a[0], a[1], a[2], a[3], y0, y1);
+            v[j] = pack_bf16x2(y0, y1);
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                           stg + lane * 64 + ((j ^ (lane >> 1)) & 3) * 16),
+                       "r"(v[4 * j]), "r"(v[4 * j + 1]), "r"(v[4 * j + 2]), "r"(v[4 * j + 3])
+                       : "memory");
+        __syncwarp();
+        const int o0 = (EPI == FVB_EPI_GEGLU ? (f0 + c) >> 1 : f0 + c) + (lane & 3) * (16 / eb);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = i * 8 + (lane >> 2);
+          uint32_t x[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                       : "r"(stg + row * 64 + (((lane & 3) ^ (row >> 1)) & 3) * 16));
+          if (t0 + row >= p.m || o0 >= nf_out) continue;
+          uint8_t* o = static_cast<uint8_t*>(p.out) + ((long long)(t0 + row) * p.ldo + o0) * eb;
+          if (p.vec_out && o0 + 16 / eb <= nf_out) {
+            *reinterpret_cast<uint4*>(o) = make_uint4(x[0], x[1], x[2], x[3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16 / eb; ++j)
+              if (o0 + j < nf_out) {
+                if (eb == 4)
+                  reinterpret_cast<uint32_t*>(o)[j] = x[j & 3];
+                else
+                  reinterpret_cast<uint16_t*>(o)[j] = (uint16_t)(x[j >> 1] >> (16 * (j & 1)));
+              }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  cluster_arrive();  // every MMA, commit and remote arrival is done
+  cluster_wait();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
 }
 
 }  // namespace g8

@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_kernel(const AttendDev p) {
     }
     for (int i = 0; i < n_tiles; ++i) {
       const int st = (cnt + i) % C::STAGES;
-      if (!mbar_wait(&full[st], ((cnt + i) / C::STAGES) & 1)) { alive = false; break; }
+      if (!mbar_wait_spin(&full[st], ((cnt + i) / C::STAGES) & 1)) { alive = false; break; }
       const uint32_t sk = ring + st * C::TILE, sv = sk + SUB * C::PITCH;
       const int nv = min(SUB, len - ((k_first + i) * UNIT + warp * SUB));
       // two chains of products, so that one does not wait for the other

@@ -73,38 +73,46 @@ int launch_norm_fp8(const fvb::n8::Dev& d, int delta, int rows, cudaStream_t st)
   return launch_norm_fp8<TX, N::DELTA_BF16>(d, rows, st);
 }
 
-template <int BN, bool SWAP, int EPI>
-int launch_gemm_fp8(const CUtensorMap& ma, const CUtensorMap& mb, const fvb::g8::Dev& d,
-                    int tiles, cudaStream_t st) {
-  using C = fvb::g8::Cfg<BN, SWAP>;
-  auto kern = fvb::g8::gemm_fp8_kernel<BN, SWAP, EPI>;
-  if (int r = ensure_smem(reinterpret_cast<const void*>(kern), C::SMEM, "fvb_gemm_fp8")) return r;
+int launch_gemm_fp8(const void* kern, const CUtensorMap& ma, const CUtensorMap& mb,
+                    const fvb::g8::Dev& d, int ctas, int cluster, int threads, int smem,
+                    cudaStream_t st) {
+  if (int r = ensure_smem(kern, smem, "fvb_gemm_fp8")) return r;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * d.cl));
-  cfg.blockDim = dim3(C::THREADS);
-  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attrs[2];
   attrs[0].id = cudaLaunchAttributeClusterDimension;
-  attrs[0].val.clusterDim.x = d.cl;
+  attrs[0].val.clusterDim.x = cluster;
   attrs[0].val.clusterDim.y = 1;
   attrs[0].val.clusterDim.z = 1;
   attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attrs[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attrs;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ma, mb, d);
+  void* args[] = {const_cast<CUtensorMap*>(&ma), const_cast<CUtensorMap*>(&mb),
+                  const_cast<fvb::g8::Dev*>(&d)};
+  cudaError_t e = cudaLaunchKernelExC(&cfg, kern, args);
   if (e != cudaSuccess)
     return fail(FVB_ERR_CUDA, "fvb_gemm_fp8: launch failed: %s", cudaGetErrorString(e));
   return check_launch("fvb_gemm_fp8");
 }
 
 template <int BN, bool SWAP>
-int launch_gemm_fp8(int epi, const CUtensorMap& ma, const CUtensorMap& mb,
-                    const fvb::g8::Dev& d, int tiles, cudaStream_t st) {
-  if (epi == FVB_EPI_BF16) return launch_gemm_fp8<BN, SWAP, FVB_EPI_BF16>(ma, mb, d, tiles, st);
-  if (epi == FVB_EPI_GEGLU) return launch_gemm_fp8<BN, SWAP, FVB_EPI_GEGLU>(ma, mb, d, tiles, st);
-  return launch_gemm_fp8<BN, SWAP, FVB_EPI_F32_STORE>(ma, mb, d, tiles, st);
+const void* cluster_kernel(int epi) {
+  namespace G = fvb::g8;
+  if (epi == FVB_EPI_BF16)
+    return reinterpret_cast<const void*>(G::gemm_fp8_cluster<BN, SWAP, FVB_EPI_BF16>);
+  if (epi == FVB_EPI_GEGLU)
+    return reinterpret_cast<const void*>(G::gemm_fp8_cluster<BN, SWAP, FVB_EPI_GEGLU>);
+  return reinterpret_cast<const void*>(G::gemm_fp8_cluster<BN, SWAP, FVB_EPI_F32_STORE>);
+}
+const void* pair_kernel(int epi) {
+  namespace G = fvb::g8;
+  if (epi == FVB_EPI_BF16) return reinterpret_cast<const void*>(G::gemm_fp8_pair<FVB_EPI_BF16>);
+  if (epi == FVB_EPI_GEGLU) return reinterpret_cast<const void*>(G::gemm_fp8_pair<FVB_EPI_GEGLU>);
+  return reinterpret_cast<const void*>(G::gemm_fp8_pair<FVB_EPI_F32_STORE>);
 }
 
 constexpr int64_t ATTEND_COUNTER_BYTES = 4096;  // one int per CTA
@@ -216,37 +224,60 @@ int fvb_gemm_fp8(const fvb_gemm_fp8_args* a, void* stream) {
     return fail(FVB_ERR_INVALID_ARG,
                 "fvb_gemm_fp8: operands must be 16B aligned with row strides in multiples of 16");
   if (a->m == 0) return FVB_OK;
-  const bool swap = a->m <= 64;
-  int bn = 128;
-  if (swap) bn = a->m <= 16 ? 16 : (a->m <= 32 ? 32 : 64);
-  const int m_side = swap ? a->n : a->m, n_side = swap ? a->m : a->n;
-  const int m_tiles = (m_side + 127) / 128, n_tiles = (n_side + bn - 1) / bn;
-  const int64_t tiles = (int64_t)m_tiles * n_tiles;
-  const int sms = sm_count();
-  int cl = 1;
-  while (cl < 8 && tiles * cl * 2 <= sms + sms / 4 && cl * 2 <= groups) cl *= 2;
-  if (tiles * cl > INT32_MAX)
-    return fail(FVB_ERR_UNSUPPORTED, "fvb_gemm_fp8: too many tiles");
-  CUtensorMap ma, mb;
-  int r = swap ? make_map_u8(&ma, a->b, a->n, a->k, a->ldb, 128)
-               : make_map_u8(&ma, a->a, a->m, a->k, a->lda, 128);
-  if (!r) r = swap ? make_map_u8(&mb, a->a, a->m, a->k, a->lda, bn)
-                   : make_map_u8(&mb, a->b, a->n, a->k, a->ldb, bn);
-  if (r) return r;
   fvb::g8::Dev d;
-  d.m = a->m; d.n = a->n; d.k = a->k;
-  d.groups = groups; d.m_tiles = m_tiles; d.cl = cl;
+  d.m = a->m; d.n = a->n; d.groups = groups;
   d.sa = a->a_scale; d.ld_sa = a->ld_as;
   d.sb = a->b_scale; d.ld_sb = a->ld_bs;
   d.out = a->out; d.ldo = a->ldo;
-  const int ob = a->epilogue == FVB_EPI_F32_STORE ? 16 : (a->epilogue == FVB_EPI_BF16 ? 8 : 4);
   const int eb = a->epilogue == FVB_EPI_F32_STORE ? 4 : 2;
-  d.vec_out = aligned(a->out, ob) && a->ldo * eb % ob == 0;
+  d.vec_out = aligned16(a->out) && a->ldo * eb % 16 == 0;
+  d.cl_log2 = 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (!swap) return launch_gemm_fp8<128, false>(a->epilogue, ma, mb, d, (int)tiles, st);
-  if (bn == 16) return launch_gemm_fp8<16, true>(a->epilogue, ma, mb, d, (int)tiles, st);
-  if (bn == 32) return launch_gemm_fp8<32, true>(a->epilogue, ma, mb, d, (int)tiles, st);
-  return launch_gemm_fp8<64, true>(a->epilogue, ma, mb, d, (int)tiles, st);
+  const int sms = sm_count();
+  // the map of an operand: boxes of 128 features, or of a tile's token rows
+  CUtensorMap mt, mf;
+  int r = make_map_u8(&mf, a->b, a->n, a->k, a->ldb, 128);
+  if (r) return r;
+  // two-SM tiles where there are enough of them
+  const int t_pair = (a->m + 255) / 256, f_pair = (a->n + 255) / 256;
+  bool pair = a->m > 128 && (int64_t)t_pair * f_pair >= sms / 2;
+  if (getenv("FVB_G8")) pair = atoi(getenv("FVB_G8"));
+  if (pair) {
+    d.t_tiles = t_pair; d.f_tiles = f_pair;
+    const int64_t tiles = (int64_t)t_pair * f_pair;
+    if (tiles > INT32_MAX / groups) return fail(FVB_ERR_UNSUPPORTED, "fvb_gemm_fp8: too large");
+    r = make_map_u8(&mt, a->a, a->m, a->k, a->lda, 128);
+    if (r) return r;
+    const int pairs = tiles < sms / 2 ? (int)tiles : sms / 2;
+    return launch_gemm_fp8(pair_kernel(a->epilogue), mt, mf, d, 2 * pairs, 2,
+                           fvb::g8::THREADS, fvb::g8::PairCfg::SMEM, st);
+  }
+  const int rows = a->m <= 16 ? 16 : (a->m <= 32 ? 32 : (a->m <= 64 ? 64 : 128));
+  const int feats = rows == 128 ? 64 : 128;
+  d.f_tiles = (a->n + feats - 1) / feats;
+  d.t_tiles = (a->m + rows - 1) / rows;
+  const int64_t tiles = (int64_t)d.f_tiles * d.t_tiles;
+  // split the groups over up to 8 CTAs while that fills SMs
+  const int fill = getenv("FVB_FILL") ? atoi(getenv("FVB_FILL")) : 2 * sms;
+  while (d.cl_log2 < 3 && (tiles << (d.cl_log2 + 1)) <= fill && (2 << d.cl_log2) <= groups)
+    ++d.cl_log2;
+  if (tiles << d.cl_log2 > INT32_MAX)
+    return fail(FVB_ERR_UNSUPPORTED, "fvb_gemm_fp8: too large");
+  r = make_map_u8(&mt, a->a, a->m, a->k, a->lda, rows);
+  if (!r && feats == 64) r = make_map_u8(&mf, a->b, a->n, a->k, a->ldb, 64);
+  if (r) return r;
+  const int ctas = (int)(tiles << d.cl_log2), cl = 1 << d.cl_log2;
+  if (rows == 16)
+    return launch_gemm_fp8(cluster_kernel<16, true>(a->epilogue), mf, mt, d, ctas, cl, fvb::g8::THREADS,
+                           fvb::g8::Cfg<16, true>::SMEM, st);
+  if (rows == 32)
+    return launch_gemm_fp8(cluster_kernel<32, true>(a->epilogue), mf, mt, d, ctas, cl, fvb::g8::THREADS,
+                           fvb::g8::Cfg<32, true>::SMEM, st);
+  if (rows == 64)
+    return launch_gemm_fp8(cluster_kernel<64, true>(a->epilogue), mf, mt, d, ctas, cl, fvb::g8::THREADS,
+                           fvb::g8::Cfg<64, true>::SMEM, st);
+  return launch_gemm_fp8(cluster_kernel<64, false>(a->epilogue), mt, mf, d, ctas, cl, fvb::g8::THREADS,
+                         fvb::g8::Cfg<64, false>::SMEM, st);
 }
 
 int fvb_paged_append(const fvb_paged_append_args* a, void* stream) {
