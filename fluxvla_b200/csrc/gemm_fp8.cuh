@@ -6,24 +6,23 @@
 // its own in TMEM and is scaled into f32 registers while the next groups'
 // products run into the others.
 //
-// TMEM lanes are the M side, and a warp reads 32 of them.  With token rows on
-// the M side a lane's factor sa * sb is one register for all its columns.
-// With the features there (SWAP: up to 64 tokens, which would leave half or
-// more of 128 rows empty) the factor varies along the columns and comes from
-// shared memory, 4 bytes for each product; that read costs 128 * BN * 4 bytes
-// of shared-memory bandwidth a group, 256 clocks at 64 tokens, less than the
-// group's weights take from HBM, but twice the MMA's own time at 128.
+// Token rows are the M side, so a TMEM lane holds one token's sums and the
+// factor sa * sb of a group is one register for all its columns.  (With the
+// features there, few tokens would not waste rows of the tensor core, but the
+// factor would vary along the columns and come from shared memory for every
+// product: 13.7 us against 11.5 us on 64 x 2048 x 16384.)
 //
-//   warp 0      TMA producer: ring of (A, B) tiles of 128-byte rows
-//   warp 1      tcgen05.mma issuer
-//   warp 2      SWAP: column factors, four groups at a time, two batches ahead
+//   warp 0      TMA producer: ring of (tokens, weights) tiles of 128-byte rows
+//   warps 1, 3  tcgen05.mma issuers, every other group each: one alone takes
+//               about 600 clocks for a group's waits, four MMAs and commits,
+//               more than a 128 x 128 product
+//   warp 2      factors, four groups at a time, two batches ahead
 //   warps 4..11 read TMEM (warp w: lanes 32*(w%4)..+31, half of the columns),
 //               multiply by the factors, accumulate
 //
 // Two kernels:
-//   gemm_fp8_cluster  one tile per CTA (128 tokens x 64 features, or 128
-//                     features x 16, 32 or 64 tokens), the groups split over
-//                     the CTAs of a cluster: enough CTAs to fill the GPU
+//   gemm_fp8_cluster  up to 128 tokens x 128 features a CTA, the groups split
+//                     over the CTAs of a cluster: enough CTAs to fill the GPU
 //                     however few the tiles are.  The partial tiles are
 //                     exchanged through distributed shared memory and summed
 //                     in the order of the groups, so a product is the same
@@ -43,14 +42,16 @@ namespace g8 {
 constexpr int GROUP = 128;
 constexpr int BATCH = 4;  // groups of one batch of column factors
 constexpr int THREADS = 384;
-constexpr int SCALE_WARP = 2, FIRST_SUM_WARP = 4;
+constexpr int FACTOR_WARP = 2, FIRST_SUM_WARP = 4;
 
 struct Dev {
   int m, n;          // tokens, features
   int groups;        // of 128 columns
   int f_tiles;       // feature tiles
   int t_tiles;       // token tiles
-  int cl_log2;       // CTAs of a cluster (gemm_fp8_cluster)
+  int cl;            // CTAs of a cluster (gemm_fp8_cluster)
+  int rows;          // tokens of a tile (gemm_fp8_cluster), a multiple of 8
+  int stages;        // of the ring (gemm_fp8_cluster)
   const float* sa;   // [tokens, groups]
   long long ld_sa;
   const float* sb;   // [features / 128, groups]
@@ -109,28 +110,33 @@ __device__ __forceinline__ uint32_t mapa(uint32_t saddr, uint32_t rank) {
   return r;
 }
 
-// 32 TMEM lanes x N columns into registers; tmem_wait makes them valid
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* r);
-template <>
-__device__ __forceinline__ void tmem_ld<8>(uint32_t taddr, uint32_t* r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
-                 "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr));
+// bounded wait with cluster-scope acquire (arrivals come from the peer too)
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t t0 = 0;
+  for (uint32_t n = 0;; ++n) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((n & 63) == 0) {
+      const uint64_t t = globaltimer_ns();
+      if (!t0) t0 = t;
+      if (t - t0 > FVB_WAIT_LIMIT_NS) {
+        record_device_error(FVB_ERR_DEVICE_TIMEOUT);
+        return false;
+      }
+    }
+  }
 }
-template <>
-__device__ __forceinline__ void tmem_ld<16>(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-        "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-template <>
-__device__ __forceinline__ void tmem_ld<32>(uint32_t taddr, uint32_t* r) {
+
+// 32 TMEM lanes x 32 columns into registers; tmem_wait makes them valid
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -151,18 +157,6 @@ __device__ __forceinline__ void tmem_wait(uint32_t* r) {
   for (int j = 0; j < N; ++j) asm volatile("" : "+r"(r[j]));
 }
 
-// acc[N] += r[N] * cs[N] (cs: 16-byte aligned shared memory, read by all lanes)
-template <int N>
-__device__ __forceinline__ void scale_add(float* acc, const uint32_t* r, const float* cs) {
-#pragma unroll
-  for (int j = 0; j < N; j += 4) {
-    const float4 s = *reinterpret_cast<const float4*>(cs + j);
-    acc[j] = fmaf(__uint_as_float(r[j]), s.x, acc[j]);
-    acc[j + 1] = fmaf(__uint_as_float(r[j + 1]), s.y, acc[j + 1]);
-    acc[j + 2] = fmaf(__uint_as_float(r[j + 2]), s.z, acc[j + 2]);
-    acc[j + 3] = fmaf(__uint_as_float(r[j + 3]), s.w, acc[j + 3]);
-  }
-}
 // acc[N] += r[N] * f
 template <int N>
 __device__ __forceinline__ void scale_add(float* acc, const uint32_t* r, float f) {
@@ -188,7 +182,7 @@ __device__ __forceinline__ void geglu2(float x0, float u0, float x1, float u1, f
   y1 = x1 * u1 * (r * d0);
 }
 
-// Writes NF consecutive features f.. of token t (NF = 4, 8 or 16; for GEGLU
+// Writes NF consecutive features f.. of token t (NF = 8; for GEGLU
 // features 2i, 2i+1 are gate and up of output i), cut at the last feature.
 template <int NF, int EPI>
 __device__ __forceinline__ void store_features(const Dev& p, int t, int f, const float (&v)[NF]) {
@@ -239,40 +233,34 @@ __device__ __forceinline__ void store_features(const Dev& p, int t, int f, const
   }
 }
 
-// The factor warp: sa * sb of token rows t0..t0+ROWS-1 and BLOCKS feature
-// blocks for the groups g0..g1, a batch of four groups at a time into
-// fac[slot][block][row][group] (or [slot][group][row], COLUMNS).  Lanes run
-// over the groups first: 16 bytes of a row are one access, where a load of
-// one group for 32 rows would touch 32 lines, and every summing warp would
-// repeat it.  bt counts batches over a CTA's tiles.
-template <int ROWS, int BLOCKS, bool COLUMNS>
+// The factor warp: sa * sb of token rows t0..t0+127 and BLOCKS feature blocks
+// for the groups g0..g1, a batch of four groups at a time into
+// fac[slot][block][row][group].  Lanes run over the groups first: 16 bytes of a
+// row are one access, where a load of one group for 32 rows would touch 32
+// lines, and every summing warp would repeat it.  bt counts batches over a
+// CTA's tiles.
+template <int BLOCKS>
 __device__ __forceinline__ bool write_factors(const Dev& p, int t0, int block, int g0, int g1,
                                               float* fac, uint64_t* ffull, uint64_t* fempty,
                                               int& bt, int lane) {
-  static_assert(!COLUMNS || BLOCKS == 1, "layout");
   const int e = lane & (BATCH - 1), r0 = lane / BATCH;
   const int last = (p.n - 1) / 128;
   for (int g = g0; g < g1; g += BATCH, ++bt) {
     const int ge = min(g + e, g1 - 1), slot = bt & 1;
-    float a[ROWS / 8], b[BLOCKS];
+    float a[16], b[BLOCKS];
 #pragma unroll
     for (int i = 0; i < BLOCKS; ++i)
       b[i] = __ldg(p.sb + (long long)min(block + i, last) * p.ld_sb + ge);
 #pragma unroll
-    for (int i = 0; i < ROWS / 8; ++i)
+    for (int i = 0; i < 16; ++i)
       a[i] = __ldg(p.sa + (long long)min(t0 + i * 8 + r0, p.m - 1) * p.ld_sa + ge);
     if (!mbar_wait(&fempty[slot], ((bt >> 1) & 1) ^ 1)) return false;
-    float* f = fac + slot * (BATCH * ROWS * BLOCKS);
+    float* f = fac + slot * (BATCH * 128 * BLOCKS);
 #pragma unroll
-    for (int i = 0; i < ROWS / 8; ++i) {
-      const int row = i * 8 + r0;
-      if (COLUMNS) {
-        f[e * ROWS + row] = a[i] * b[0];
-      } else {
+    for (int i = 0; i < 16; ++i)
 #pragma unroll
-        for (int j = 0; j < BLOCKS; ++j) f[(j * ROWS + row) * BATCH + e] = a[i] * b[j];
-      }
-    }
+      for (int j = 0; j < BLOCKS; ++j)
+        f[(j * 128 + i * 8 + r0) * BATCH + e] = a[i] * b[j];
     __syncwarp();
     if (lane == 0) mbar_arrive(&ffull[slot]);
   }
@@ -285,56 +273,64 @@ __device__ __forceinline__ float pick(const float4& v, int e) {
 // ---------------------------------------------------------------------------
 // one tile per CTA, groups split over a cluster
 // ---------------------------------------------------------------------------
-template <int BN, bool SWAP>
-struct Cfg {
-  static_assert(BN <= 64, "two CTAs share an SM's TMEM and registers");
-  static constexpr int A_BYTES = 128 * GROUP;
-  static constexpr int STAGE = A_BYTES + BN * GROUP;
-  static constexpr int STAGES = BN == 16 ? 5 : (BN == 32 ? 4 : 3);
-  static constexpr int NB = 4;                       // accumulators
-  static constexpr int COLS = BN / 2;                // columns of a warp
-  static constexpr uint32_t TMEM_COLS = NB * BN;
-  // partials [tokens][features] f32; rows written lane by lane are padded
-  static constexpr int T_ROWS = SWAP ? BN : 128, F_COLS = SWAP ? 128 : BN;
-  static constexpr int PITCH = SWAP ? 128 : BN + 4;
-  static constexpr int OFF_RECV = STAGES * STAGE;
-  static constexpr int OFF_CS = OFF_RECV + T_ROWS * PITCH * 4;
-  static constexpr int OFF_BAR = OFF_CS + 2 * BATCH * T_ROWS * 4;
-  static constexpr int SMEM = OFF_BAR + (2 * STAGES + 2 * NB + 4) * 8 + 16 + 1024;
+struct ClusterCfg {
+  static constexpr int TILE = 128;                  // features (and most tokens)
+  static constexpr int B_BYTES = TILE * GROUP;
+  static constexpr int NB = 4;                      // accumulators
+  static constexpr int COLS = TILE / 2;             // features of a warp
+  static constexpr int PITCH = TILE + 4;            // floats of a partial row
+  static constexpr int MAX_STAGES = 12;
+  static constexpr int MAX_SMEM = 232448;           // of a CTA
+  static constexpr int FAC = 2 * BATCH * TILE * 4;
+  static constexpr int BARS = (2 * MAX_STAGES + 2 * NB + 5) * 8 + 16;
+  // [ring][partials received: up to rows + 8 x PITCH f32][factors][barriers]
+  __host__ __device__ static constexpr int stage_bytes(int rows) { return rows * GROUP + B_BYTES; }
+  __host__ __device__ static constexpr int part_bytes(int rows) { return rows * PITCH * 4; }
+  static constexpr int fixed_bytes(int rows) {
+    return part_bytes(rows + 8) + FAC + BARS + 1024;
+  }
+  static int stages(int rows) {
+    const int s = (MAX_SMEM - fixed_bytes(rows)) / stage_bytes(rows);
+    return s < MAX_STAGES ? s : MAX_STAGES;
+  }
+  static int smem(int rows) { return fixed_bytes(rows) + stages(rows) * stage_bytes(rows); }
 };
 
-template <int BN, bool SWAP, int EPI>
-__global__ void __launch_bounds__(THREADS, 2)
+template <int EPI>
+__global__ void __launch_bounds__(THREADS, 1)
     gemm_fp8_cluster(const __grid_constant__ CUtensorMap tmA,
                      const __grid_constant__ CUtensorMap tmB, const Dev p) {
-  using C = Cfg<BN, SWAP>;
+  using C = ClusterCfg;
   constexpr int COLS = C::COLS, NB = C::NB;
-  constexpr int LD = COLS < 32 ? COLS : 32;  // columns of one TMEM read
-  constexpr uint32_t IDESC = idesc_e4m3_f32(128, BN);
+  constexpr uint32_t IDESC = idesc_e4m3_f32(128, C::TILE);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* cs = reinterpret_cast<float*>(smem + C::OFF_CS);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  uint64_t* empty = full + C::STAGES;
-  uint64_t* tfull = empty + C::STAGES;  // [NB]
-  uint64_t* tempty = tfull + NB;        // [NB]
-  uint64_t* csfull = tempty + NB;       // [2]
-  uint64_t* csempty = csfull + 2;       // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(csempty + 2);
+  const int rows = p.rows, stages = p.stages;
+  const int a_bytes = rows * GROUP, stage_bytes = a_bytes + C::B_BYTES;
+  uint8_t* recv = smem + stages * stage_bytes;
+  float* fac = reinterpret_cast<float*>(recv + C::part_bytes(rows + 8));
+  uint64_t* full = reinterpret_cast<uint64_t*>(fac + C::FAC / 4);
+  uint64_t* empty = full + C::MAX_STAGES;
+  uint64_t* tfull = empty + C::MAX_STAGES;  // [NB]
+  uint64_t* tempty = tfull + NB;            // [NB]
+  uint64_t* ffull = tempty + NB;            // [2]
+  uint64_t* fempty = ffull + 2;             // [2]
+  uint64_t* recvd = fempty + 2;             // the cluster's partials are here
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(recvd + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cl = 1 << p.cl_log2;
-  const uint32_t rank = cl > 1 ? cluster_rank() : 0;
-  const int tile = blockIdx.x >> p.cl_log2;
-  const int ft = tile % p.f_tiles, tt = tile / p.f_tiles;
-  const int f0 = ft * C::F_COLS, t0 = tt * C::T_ROWS;
-  const int g0 = (int)(((long long)p.groups * rank) >> p.cl_log2);
-  const int g1 = (int)(((long long)p.groups * (rank + 1)) >> p.cl_log2);
+  const int cl = p.cl;
+  const int rank = cl > 1 ? (int)cluster_rank() : 0;
+  const int tile = blockIdx.x / cl;
+  const int f0 = tile % p.f_tiles * C::TILE, t0 = tile / p.f_tiles * rows;
+  const int g0 = (int)((long long)p.groups * rank / cl);
+  const int g1 = (int)((long long)p.groups * (rank + 1) / cl);
   const int ng = g1 - g0;
-  const int per = C::T_ROWS >> p.cl_log2;  // token rows that each CTA sums
+  // token rows that this CTA sums
+  const int my0 = rows * rank / cl, per = rows * (rank + 1) / cl - my0;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -343,62 +339,80 @@ __global__ void __launch_bounds__(THREADS, 2)
       mbar_init(&tempty[a], 8);
     }
     for (int a = 0; a < 2; ++a) {
-      mbar_init(&csfull[a], 1);
-      mbar_init(&csempty[a], 8);
+      mbar_init(&ffull[a], 1);
+      mbar_init(&fempty[a], 8);
     }
+    mbar_init(recvd, 1);
     fence_barrier_init();
+    mbar_arrive_expect_tx(recvd, cl * C::part_bytes(per));
     prefetch_tensormap(&tmA);
     prefetch_tensormap(&tmB);
   }
-  if (warp == 1) tmem_alloc(tmem_slot, C::TMEM_COLS);
+  if (warp == 1) tmem_alloc(tmem_slot, NB * C::TILE);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (cl > 1) cluster_arrive();  // waited for before the first remote store
+  if (cl > 1) cluster_arrive();  // waited for before the first remote copy
   const uint32_t tmem = *tmem_slot;
   griddep_wait();
   griddep_launch_dependents();
 
   if (warp == 0) {
     if (lane == 0) {
+      int s = 0;
+      uint32_t phase = 1;
       for (int i = 0; i < ng; ++i) {
-        const int s = i % C::STAGES;
-        if (!mbar_wait_spin(&empty[s], ((i / C::STAGES) & 1) ^ 1)) break;
-        mbar_arrive_expect_tx(&full[s], C::STAGE);
-        uint8_t* sa = smem + s * C::STAGE;
-        tma_load_2d(sa, &tmA, (g0 + i) * GROUP, SWAP ? f0 : t0, &full[s]);
-        tma_load_2d(sa + C::A_BYTES, &tmB, (g0 + i) * GROUP, SWAP ? t0 : f0, &full[s]);
+        if (!mbar_wait_spin(&empty[s], phase)) break;
+        mbar_arrive_expect_tx(&full[s], stage_bytes);
+        uint8_t* st = smem + s * stage_bytes;
+        tma_load_2d(st + a_bytes, &tmB, (g0 + i) * GROUP, f0, &full[s]);
+        tma_load_2d(st, &tmA, (g0 + i) * GROUP, t0, &full[s]);
+        if (++s == stages) {
+          s = 0;
+          phase ^= 1;
+        }
       }
     }
     __syncwarp();
     if (cl > 1) cluster_wait();
-  } else if (warp == 1) {
+  } else if (warp == 1 || warp == 3) {
+    // a tile of fewer than 128 rows: the MMA reads on into the weights, which
+    // makes sums in lanes that nobody reads
     const bool elected = elect_one();
-    for (int i = 0; i < ng; ++i) {
-      const int s = i % C::STAGES, b = i % NB;
-      bool ready = mbar_wait_spin(&full[s], (i / C::STAGES) & 1);
+    const int first = warp >> 1;
+    int s = first % stages;
+    uint32_t phase = (first / stages) & 1;
+#pragma unroll 1
+    for (int i = first; i < ng; i += 2) {
+      const int b = i % NB;
+      bool ready = mbar_wait_spin(&full[s], phase);
       ready = ready && mbar_wait_spin(&tempty[b], ((i / NB) & 1) ^ 1);
       if (!__all_sync(0xffffffffu, ready)) break;
       tc_fence_after();
       if (elected) {
-        const uint64_t da = smem_desc_sw128(smem_u32(smem + s * C::STAGE));
-        const uint64_t db = smem_desc_sw128(smem_u32(smem + s * C::STAGE + C::A_BYTES));
+        const uint64_t da = smem_desc_sw128(smem_u32(smem + s * stage_bytes));
+        const uint64_t db = smem_desc_sw128(smem_u32(smem + s * stage_bytes + a_bytes));
 #pragma unroll
         for (int kk = 0; kk < GROUP / 32; ++kk)
-          mma_e4m3<1>(tmem + b * BN, da + kk * 2, db + kk * 2, IDESC, kk > 0);
+          mma_e4m3<1>(tmem + b * C::TILE, da + kk * 2, db + kk * 2, IDESC, kk > 0);
         tc_commit(&tfull[b]);
         tc_commit(&empty[s]);
       }
       __syncwarp();
+      s += 2;
+      if (s >= stages) {
+        s -= stages;
+        phase ^= 1;
+      }
     }
     if (cl > 1) cluster_wait();
-  } else if (warp < FIRST_SUM_WARP) {
+  } else if (warp == FACTOR_WARP) {
     int bt = 0;
-    if (warp == SCALE_WARP)
-      write_factors<C::T_ROWS, 1, SWAP>(p, t0, f0 / 128, g0, g1, cs, csfull, csempty, bt, lane);
+    write_factors<1>(p, t0, f0 / 128, g0, g1, fac, ffull, fempty, bt, lane);
     if (cl > 1) cluster_wait();
   } else {
     const int q = warp & 3, half = (warp - FIRST_SUM_WARP) >> 2;
+    const bool used = q * 32 < rows;  // lanes past the last row are not read
     float acc[COLS];
 #pragma unroll
     for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
@@ -406,13 +420,10 @@ __global__ void __launch_bounds__(THREADS, 2)
     bool ok = true;
     for (int i0 = 0; i0 < ng && ok; i0 += BATCH) {
       const int slot = (i0 / BATCH) & 1;
-      ok = mbar_wait_spin(&csfull[slot], (i0 / (2 * BATCH)) & 1);
-      float4 f4;
-      if (!SWAP) {
-        f4 = reinterpret_cast<const float4*>(cs)[slot * 128 + q * 32 + lane];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&csempty[slot]);
-      }
+      ok = mbar_wait_spin(&ffull[slot], (i0 / (2 * BATCH)) & 1);
+      const float4 f4 = reinterpret_cast<const float4*>(fac)[slot * 128 + q * 32 + lane];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&fempty[slot]);
 #pragma unroll
       for (int e = 0; e < BATCH; ++e) {
         const int i = i0 + e, b = i % NB;
@@ -421,86 +432,77 @@ __global__ void __launch_bounds__(THREADS, 2)
           ok = __all_sync(0xffffffffu, ok);
           if (ok) {
             tc_fence_after();
-            const uint32_t ta = lane_base + b * BN;
             uint32_t r[COLS];
+            if (used) {
 #pragma unroll
-            for (int j = 0; j < COLS; j += LD) tmem_ld<LD>(ta + j, r + j);
-            tmem_wait<COLS>(r);
+              for (int j = 0; j < COLS; j += 32) tmem_ld32(lane_base + b * C::TILE + j, r + j);
+              tmem_wait<COLS>(r);
+            }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&tempty[b]);
-            if (SWAP)
-              scale_add<COLS>(acc, r, cs + (slot * BATCH + e) * BN + half * COLS);
-            else
-              scale_add<COLS>(acc, r, pick(f4, e));
+            if (used) scale_add<COLS>(acc, r, pick(f4, e));
           }
         }
       }
-      __syncwarp();
-      if (SWAP && lane == 0) mbar_arrive(&csempty[slot]);
     }
-    // each token row goes to the CTA that sums it
-    if (cl > 1) cluster_wait();
-    if (ok) {
-      const uint32_t recv = smem_u32(smem + C::OFF_RECV);
-      if (SWAP) {
-        // columns are tokens: 32 lanes hold 32 features of one
+    // every product has been read, so the ring is free: the partial tile goes
+    // there, and each CTA's token rows in one copy to that CTA
+    if (q * 32 + lane < rows) {
+      float* t = reinterpret_cast<float*>(smem) + (q * 32 + lane) * C::PITCH + half * COLS;
 #pragma unroll
-        for (int j = 0; j < COLS; ++j) {
-          const int tok = half * COLS + j;
-          const uint32_t at =
-              recv + ((rank * per + (tok & (per - 1))) * C::PITCH + q * 32 + lane) * 4;
-          if (cl > 1)
-            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa(at, tok / per)),
-                         "f"(acc[j])
-                         : "memory");
-          else
-            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(acc[j]) : "memory");
-        }
-      } else {
-        const int tok = q * 32 + lane;
-        uint32_t at =
-            recv + ((rank * per + (tok & (per - 1))) * C::PITCH + half * COLS) * 4;
-        if (cl > 1) at = mapa(at, tok / per);
-#pragma unroll
-        for (int j = 0; j < COLS; j += 4) {
-          if (cl > 1)
-            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + j * 4),
-                         "f"(acc[j]), "f"(acc[j + 1]), "f"(acc[j + 2]), "f"(acc[j + 3])
-                         : "memory");
-          else
-            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + j * 4),
-                         "f"(acc[j]), "f"(acc[j + 1]), "f"(acc[j + 2]), "f"(acc[j + 3])
-                         : "memory");
-        }
+      for (int j = 0; j < COLS; j += 4)
+        *reinterpret_cast<float4*>(t + j) =
+            make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+    }
+    fence_proxy_async_smem();
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (cl > 1) {
+      cluster_wait();
+      if (warp == FIRST_SUM_WARP && lane < cl && ok) {
+        const int to = rows * lane / cl;  // first row of the CTA that this lane serves
+        const uint32_t bytes = C::part_bytes(rows * (lane + 1) / cl - to);
+        asm volatile(
+            "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes "
+            "[%0], [%1], %2, [%3];" ::"r"(mapa(smem_u32(recv) + rank * bytes, lane)),
+            "r"(smem_u32(smem) + C::part_bytes(to)), "r"(bytes), "r"(mapa(smem_u32(recvd), lane))
+            : "memory");
       }
     }
   }
   tc_fence_before();
-  __syncwarp();
-  if (cl > 1) {
-    cluster_arrive();
-    cluster_wait();
-  } else {
-    __syncthreads();
-  }
+  __syncthreads();
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, C::TMEM_COLS);
+    tmem_dealloc(tmem, NB * C::TILE);
   }
   // this CTA's tokens: the cluster's partials in the order of the groups
-  const float* recv = reinterpret_cast<const float*>(smem + C::OFF_RECV);
-#pragma unroll 4
-  for (int e = threadIdx.x; e < per * (C::F_COLS / 4); e += THREADS) {
-    const int r = e / (C::F_COLS / 4), f = e % (C::F_COLS / 4) * 4;
-    float4 v = *reinterpret_cast<const float4*>(recv + r * C::PITCH + f);
+  const float* part = reinterpret_cast<const float*>(cl > 1 ? recv : smem);
+  if (cl > 1) mbar_wait_cluster(recvd, 0);
+  constexpr int NF = 8;
+#pragma unroll 2
+  for (int e = threadIdx.x; e < per * (C::TILE / NF); e += THREADS) {
+    const int r = e / (C::TILE / NF), f = e % (C::TILE / NF) * NF;
+    float v[NF];
+#pragma unroll
+    for (int j = 0; j < NF; j += 4)
+      *reinterpret_cast<float4*>(v + j) =
+          *reinterpret_cast<const float4*>(part + r * C::PITCH + f + j);
     for (int i = 1; i < cl; ++i) {
-      const float4 w = *reinterpret_cast<const float4*>(recv + (i * per + r) * C::PITCH + f);
-      v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+#pragma unroll
+      for (int j = 0; j < NF; j += 4) {
+        const float4 w =
+            *reinterpret_cast<const float4*>(part + (i * per + r) * C::PITCH + f + j);
+        v[j] += w.x; v[j + 1] += w.y; v[j + 2] += w.z; v[j + 3] += w.w;
+      }
     }
-    const float y[4] = {v.x, v.y, v.z, v.w};
-    store_features<4, EPI>(p, t0 + rank * per + r, f0 + f, y);
+    store_features<NF, EPI>(p, t0 + my0 + r, f0 + f, v);
+  }
+  if (cl > 1) {
+    // the copies out of this CTA have been received everywhere
+    cluster_arrive();
+    cluster_wait();
   }
 }
 
@@ -542,31 +544,6 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster)
                : "memory");
 }
-// bounded wait with cluster-scope acquire (arrivals come from the peer too)
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
-  const uint32_t addr = smem_u32(bar);
-  uint64_t t0 = 0;
-  for (uint32_t n = 0;; ++n) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(addr), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if ((n & 63) == 0) {
-      const uint64_t t = globaltimer_ns();
-      if (!t0) t0 = t;
-      if (t - t0 > FVB_WAIT_LIMIT_NS) {
-        record_device_error(FVB_ERR_DEVICE_TIMEOUT);
-        return false;
-      }
-    }
-  }
-}
-
 template <int EPI>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_fp8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -641,15 +618,15 @@ __global__ void __launch_bounds__(THREADS, 1)
           tma_load_2d_pair(sa + C::HALF, &tmB, g * GROUP, wrow, fb);
         }
       }
-    } else if (warp == 1 && rank == 0) {
-      const bool elected = elect_one();
+    } else if ((warp == 1 || warp == 3) && rank == 0) {
       constexpr uint32_t IDESC = idesc_e4m3_f32(256, C::TILE);
+      const bool elected = elect_one();
       const int n_it = p.groups * ((n_tiles - pair + n_pairs - 1) / n_pairs);
-      int s = 0;
+      const int b = warp >> 1;  // accumulator of this issuer's groups
+      int s = b;
       uint32_t phase = 0;
 #pragma unroll 1
-      for (int it = 0; it < n_it; ++it) {
-        const int b = it & 1;
+      for (int it = b; it < n_it; it += 2) {
         bool ready = mbar_wait_spin(&full[s], phase);
         ready = ready && mbar_wait_cluster(&tempty[b], ((it >> 1) & 1) ^ 1);
         if (!__all_sync(0xffffffffu, ready)) break;
@@ -664,18 +641,18 @@ __global__ void __launch_bounds__(THREADS, 1)
           commit_both(&empty[s]);
         }
         __syncwarp();
-        if (++s == C::STAGES) {
-          s = 0;
+        s += 2;
+        if (s >= C::STAGES) {
+          s -= C::STAGES;
           phase ^= 1;
         }
       }
-    } else if (warp == SCALE_WARP) {
+    } else if (warp == FACTOR_WARP) {
       int bt = 0;
       bool alive = true;
       for (int w = pair; w < n_tiles && alive; w += n_pairs)
-        alive = write_factors<128, 2, false>(p, (w % p.t_tiles) * C::TILE + (int)rank * 128,
-                                             (w / p.t_tiles) * 2, 0, p.groups, fac, ffull, fempty,
-                                             bt, lane);
+        alive = write_factors<2>(p, (w % p.t_tiles) * C::TILE + (int)rank * 128,
+                                 (w / p.t_tiles) * 2, 0, p.groups, fac, ffull, fempty, bt, lane);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -710,12 +687,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_fence_after();
         const uint32_t ta = lane_base + b * C::TILE;
         uint32_t r[2][32];
-        tmem_ld<32>(ta, r[0]);
+        tmem_ld32(ta, r[0]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           tmem_wait<32>(r[j & 1]);
           if (j < 3) {
-            tmem_ld<32>(ta + 32 * j + 32, r[(j + 1) & 1]);
+            tmem_ld32(ta + 32 * j + 32, r[(j + 1) & 1]);
           } else {
             tc_fence_before();
             __syncwarp();

@@ -74,12 +74,11 @@ int launch_norm_fp8(const fvb::n8::Dev& d, int delta, int rows, cudaStream_t st)
 }
 
 int launch_gemm_fp8(const void* kern, const CUtensorMap& ma, const CUtensorMap& mb,
-                    const fvb::g8::Dev& d, int ctas, int cluster, int threads, int smem,
-                    cudaStream_t st) {
-  if (int r = ensure_smem(kern, smem, "fvb_gemm_fp8")) return r;
+                    const fvb::g8::Dev& d, int ctas, int cluster, int smem, cudaStream_t st) {
+  if (int r = ensure_smem(kern, fvb::g8::ClusterCfg::MAX_SMEM, "fvb_gemm_fp8")) return r;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(threads);
+  cfg.blockDim = dim3(fvb::g8::THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attrs[2];
@@ -99,20 +98,49 @@ int launch_gemm_fp8(const void* kern, const CUtensorMap& ma, const CUtensorMap& 
   return check_launch("fvb_gemm_fp8");
 }
 
-template <int BN, bool SWAP>
 const void* cluster_kernel(int epi) {
   namespace G = fvb::g8;
-  if (epi == FVB_EPI_BF16)
-    return reinterpret_cast<const void*>(G::gemm_fp8_cluster<BN, SWAP, FVB_EPI_BF16>);
+  if (epi == FVB_EPI_BF16) return reinterpret_cast<const void*>(G::gemm_fp8_cluster<FVB_EPI_BF16>);
   if (epi == FVB_EPI_GEGLU)
-    return reinterpret_cast<const void*>(G::gemm_fp8_cluster<BN, SWAP, FVB_EPI_GEGLU>);
-  return reinterpret_cast<const void*>(G::gemm_fp8_cluster<BN, SWAP, FVB_EPI_F32_STORE>);
+    return reinterpret_cast<const void*>(G::gemm_fp8_cluster<FVB_EPI_GEGLU>);
+  return reinterpret_cast<const void*>(G::gemm_fp8_cluster<FVB_EPI_F32_STORE>);
 }
 const void* pair_kernel(int epi) {
   namespace G = fvb::g8;
   if (epi == FVB_EPI_BF16) return reinterpret_cast<const void*>(G::gemm_fp8_pair<FVB_EPI_BF16>);
   if (epi == FVB_EPI_GEGLU) return reinterpret_cast<const void*>(G::gemm_fp8_pair<FVB_EPI_GEGLU>);
   return reinterpret_cast<const void*>(G::gemm_fp8_pair<FVB_EPI_F32_STORE>);
+}
+
+// Clusters of 1..8 CTAs of the cluster kernel (one CTA per SM) that the device
+// runs at once: fewer than its SMs over the size, since a cluster stays in one
+// GPC (148, 74, 45, 33, 26, 22, 15, 15 on a B200).
+const int* cluster_slots() {
+  static std::mutex mu;
+  static int slots[128][9] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) dev = 0;
+  std::lock_guard<std::mutex> lk(mu);
+  if (slots[dev][1]) return slots[dev];
+  const void* kern = cluster_kernel(FVB_EPI_BF16);
+  for (int c = 8; c >= 1; --c) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c * 256);
+    cfg.blockDim = dim3(fvb::g8::THREADS);
+    cfg.dynamicSmemBytes = fvb::g8::ClusterCfg::MAX_SMEM;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = c;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0;
+    cudaGetLastError();
+    slots[dev][c] = n > 0 ? n : (c == 1 ? sm_count() : 0);
+  }
+  return slots[dev];
 }
 
 constexpr int64_t ATTEND_COUNTER_BYTES = 4096;  // one int per CTA
@@ -231,53 +259,54 @@ int fvb_gemm_fp8(const fvb_gemm_fp8_args* a, void* stream) {
   d.out = a->out; d.ldo = a->ldo;
   const int eb = a->epilogue == FVB_EPI_F32_STORE ? 4 : 2;
   d.vec_out = aligned16(a->out) && a->ldo * eb % 16 == 0;
-  d.cl_log2 = 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int sms = sm_count();
-  // the map of an operand: boxes of 128 features, or of a tile's token rows
+  // The shape with the least time by a count of clocks, fitted to measured
+  // products: a group costs the cluster kernel 600 clocks and a tile 4500
+  // (6000 with an exchange), the pair kernel 970 and 3500 for a tile of twice
+  // the height and width.  816 x 32768 x 2048: pair 70 us, clusters 109 us;
+  // 816 x 2560 x 2048: the other way round, 40 pair tiles leave SMs idle.
+  const void* kern = cluster_kernel(a->epilogue);
+  if (int rr = ensure_smem(kern, fvb::g8::ClusterCfg::MAX_SMEM, "fvb_gemm_fp8")) return rr;
+  if (int rr = ensure_smem(cluster_kernel(FVB_EPI_BF16), fvb::g8::ClusterCfg::MAX_SMEM,
+                           "fvb_gemm_fp8"))
+    return rr;
+  const int* slots = cluster_slots();
+  const int64_t f_tiles = (a->n + 127) / 128, t_tiles = (a->m + 127) / 128;
+  const int64_t tiles = f_tiles * t_tiles;
+  const int64_t f_pair = (a->n + 255) / 256, t_pair = (a->m + 255) / 256;
+  auto waves = [](int64_t n, int64_t at_once) { return (n + at_once - 1) / at_once; };
+  int64_t best = INT64_MAX;
+  d.cl = 1;
+  for (int c = 1; c <= 8 && c <= groups; ++c) {
+    if (!slots[c]) continue;
+    const int64_t t = waves(tiles, slots[c]) * ((groups + c - 1) / c * 600 + (c > 1 ? 6000 : 4500));
+    if (t < best) {
+      best = t;
+      d.cl = c;
+    }
+  }
+  const bool pair = slots[2] && waves(f_pair * t_pair, slots[2]) * (groups * 970ll + 3500) < best;
+  const int64_t most = INT32_MAX / 8 / groups;
+  if (tiles > most) return fail(FVB_ERR_UNSUPPORTED, "fvb_gemm_fp8: too large");
   CUtensorMap mt, mf;
   int r = make_map_u8(&mf, a->b, a->n, a->k, a->ldb, 128);
   if (r) return r;
-  // two-SM tiles where there are enough of them
-  const int t_pair = (a->m + 255) / 256, f_pair = (a->n + 255) / 256;
-  bool pair = a->m > 128 && (int64_t)t_pair * f_pair >= sms / 2;
-  if (getenv("FVB_G8")) pair = atoi(getenv("FVB_G8"));
   if (pair) {
-    d.t_tiles = t_pair; d.f_tiles = f_pair;
-    const int64_t tiles = (int64_t)t_pair * f_pair;
-    if (tiles > INT32_MAX / groups) return fail(FVB_ERR_UNSUPPORTED, "fvb_gemm_fp8: too large");
+    d.t_tiles = (int)t_pair; d.f_tiles = (int)f_pair;
     r = make_map_u8(&mt, a->a, a->m, a->k, a->lda, 128);
     if (r) return r;
-    const int pairs = tiles < sms / 2 ? (int)tiles : sms / 2;
+    const int pairs = (int)(f_pair * t_pair < slots[2] ? f_pair * t_pair : slots[2]);
     return launch_gemm_fp8(pair_kernel(a->epilogue), mt, mf, d, 2 * pairs, 2,
-                           fvb::g8::THREADS, fvb::g8::PairCfg::SMEM, st);
+                           fvb::g8::PairCfg::SMEM, st);
   }
-  const int rows = a->m <= 16 ? 16 : (a->m <= 32 ? 32 : (a->m <= 64 ? 64 : 128));
-  const int feats = rows == 128 ? 64 : 128;
-  d.f_tiles = (a->n + feats - 1) / feats;
-  d.t_tiles = (a->m + rows - 1) / rows;
-  const int64_t tiles = (int64_t)d.f_tiles * d.t_tiles;
-  // split the groups over up to 8 CTAs while that fills SMs
-  const int fill = getenv("FVB_FILL") ? atoi(getenv("FVB_FILL")) : 2 * sms;
-  while (d.cl_log2 < 3 && (tiles << (d.cl_log2 + 1)) <= fill && (2 << d.cl_log2) <= groups)
-    ++d.cl_log2;
-  if (tiles << d.cl_log2 > INT32_MAX)
-    return fail(FVB_ERR_UNSUPPORTED, "fvb_gemm_fp8: too large");
-  r = make_map_u8(&mt, a->a, a->m, a->k, a->lda, rows);
-  if (!r && feats == 64) r = make_map_u8(&mf, a->b, a->n, a->k, a->ldb, 64);
+  // tiles of equal height
+  d.f_tiles = (int)f_tiles; d.t_tiles = (int)t_tiles;
+  d.rows = (int)((a->m + t_tiles - 1) / t_tiles + 7) / 8 * 8;
+  d.stages = fvb::g8::ClusterCfg::stages(d.rows);
+  r = make_map_u8(&mt, a->a, a->m, a->k, a->lda, d.rows);
   if (r) return r;
-  const int ctas = (int)(tiles << d.cl_log2), cl = 1 << d.cl_log2;
-  if (rows == 16)
-    return launch_gemm_fp8(cluster_kernel<16, true>(a->epilogue), mf, mt, d, ctas, cl, fvb::g8::THREADS,
-                           fvb::g8::Cfg<16, true>::SMEM, st);
-  if (rows == 32)
-    return launch_gemm_fp8(cluster_kernel<32, true>(a->epilogue), mf, mt, d, ctas, cl, fvb::g8::THREADS,
-                           fvb::g8::Cfg<32, true>::SMEM, st);
-  if (rows == 64)
-    return launch_gemm_fp8(cluster_kernel<64, true>(a->epilogue), mf, mt, d, ctas, cl, fvb::g8::THREADS,
-                           fvb::g8::Cfg<64, true>::SMEM, st);
-  return launch_gemm_fp8(cluster_kernel<64, false>(a->epilogue), mt, mf, d, ctas, cl, fvb::g8::THREADS,
-                         fvb::g8::Cfg<64, false>::SMEM, st);
+  return launch_gemm_fp8(kern, mt, mf, d, (int)tiles * d.cl, d.cl,
+                         fvb::g8::ClusterCfg::smem(d.rows), st);
 }
 
 int fvb_paged_append(const fvb_paged_append_args* a, void* stream) {
