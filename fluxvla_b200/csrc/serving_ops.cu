@@ -143,7 +143,7 @@ const int* cluster_slots() {
   return slots[dev];
 }
 
-constexpr int64_t ATTEND_COUNTER_BYTES = 4096;  // one int per CTA
+constexpr int64_t ATTEND_COUNTER_BYTES = 4096;  // three ints per CTA
 
 // Launch shape of an attention call: blocks of 8 or 16 heads, one CTA per SM.
 struct AttendShape {
@@ -163,7 +163,7 @@ int attend_prepare(const fvb_paged_attn_args* a, AttendShape* s) {
   const int group = a->heads / a->kv_heads;
   s->nt = group <= 8 ? 1 : 2;
   s->head_blocks = (group + 8 * s->nt - 1) / (8 * s->nt);
-  s->ctas = sm_count() < 1024 ? sm_count() : 1024;
+  s->ctas = sm_count() < 340 ? sm_count() : 340;
   const int64_t rows = 2ll * s->ctas * 8 * s->nt;
   // the counters keep their place whatever the shape, so that calls of
   // several shapes may share a workspace one after the other
@@ -173,14 +173,45 @@ int attend_prepare(const fvb_paged_attn_args* a, AttendShape* s) {
   return FVB_OK;
 }
 
-template <int D, int NT>
-int launch_attend(const fvb::paged::AttendDev& d, int ctas, cudaStream_t st) {
-  using C = fvb::paged::Cfg<D, NT>;
-  auto kern = fvb::paged::attend_kernel<D, NT>;
+// Tensor map of a paged cache, box of 16 rows x 64 dims of one head and page.
+// Strides of a dimension of size 1 mean nothing and may be anything.
+bool make_cache_map(CUtensorMap* m, const void* ptr, int dim, int page_size, int kv_heads,
+                    int n_pages, int64_t row, int64_t head, int64_t page) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) return false;
+  if (kv_heads == 1) head = dim;
+  if (n_pages == 1) page = dim;
+  if (row <= 0 || head <= 0 || page <= 0) return false;
+  cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)page_size, (cuuint64_t)kv_heads,
+                        (cuuint64_t)n_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)head * 2, (cuuint64_t)page * 2};
+  cuuint32_t box[4] = {64, 16, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, int NT, bool BOXES>
+int launch_attend(const CUtensorMap& mk, const CUtensorMap& mv, const fvb::paged::AttendDev& d,
+                  int ctas, cudaStream_t st) {
+  using C = fvb::paged::Cfg<D, NT, BOXES>;
+  auto kern = fvb::paged::attend_kernel<D, NT, BOXES>;
   if (int r = ensure_smem(reinterpret_cast<const void*>(kern), C::SMEM, "fvb_paged_attention"))
     return r;
   return launch_k("fvb_paged_attention", kern, dim3(ctas), dim3(fvb::paged::THREADS),
-                  (size_t)C::SMEM, st, d);
+                  (size_t)C::SMEM, st, mk, mv, d);
+}
+
+template <int D>
+int launch_attend(int nt, bool boxes, const CUtensorMap& mk, const CUtensorMap& mv,
+                  const fvb::paged::AttendDev& d, int ctas, cudaStream_t st) {
+  if (boxes)
+    return nt == 1 ? launch_attend<D, 1, true>(mk, mv, d, ctas, st)
+                   : launch_attend<D, 2, true>(mk, mv, d, ctas, st);
+  return nt == 1 ? launch_attend<D, 1, false>(mk, mv, d, ctas, st)
+                 : launch_attend<D, 2, false>(mk, mv, d, ctas, st);
 }
 
 }  // namespace
@@ -369,6 +400,10 @@ int fvb_paged_attention(const fvb_paged_attn_args* a, void* stream) {
   if (max_len > INT32_MAX - 64)
     return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attention: %lld keys a sequence",
                 (long long)max_len);
+  // units of 128 keys over all sequences and heads are counted in 32 bits
+  if ((max_len / 128 + 1) * a->batch > INT32_MAX / (a->kv_heads * s.head_blocks))
+    return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attention: %d sequences of up to %lld keys",
+                a->batch, (long long)max_len);
   const int64_t s8[] = {a->kc_page_stride, a->kc_row_stride, a->kc_head_stride,
                         a->vc_page_stride, a->vc_row_stride, a->vc_head_stride};
   bool ok = aligned16(a->k_cache) && aligned16(a->v_cache);
@@ -401,11 +436,18 @@ int fvb_paged_attention(const fvb_paged_attn_args* a, void* stream) {
   d.part_o = (float*)((char*)a->workspace + s.off_o);
   d.part_ml = (float*)((char*)a->workspace + s.off_ml);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (a->head_dim == 256)
-    return s.nt == 1 ? launch_attend<256, 1>(d, s.ctas, st) : launch_attend<256, 2>(d, s.ctas, st);
-  if (a->head_dim == 128)
-    return s.nt == 1 ? launch_attend<128, 1>(d, s.ctas, st) : launch_attend<128, 2>(d, s.ctas, st);
-  return s.nt == 1 ? launch_attend<64, 1>(d, s.ctas, st) : launch_attend<64, 2>(d, s.ctas, st);
+  CUtensorMap mk, mv;
+  memset(&mk, 0, sizeof(mk));
+  memset(&mv, 0, sizeof(mv));
+  const bool boxes =
+      a->page_size % 16 == 0 && a->n_pages > 0 &&
+      make_cache_map(&mk, a->k_cache, a->head_dim, a->page_size, a->kv_heads, a->n_pages, s8[1],
+                     s8[2], s8[0]) &&
+      make_cache_map(&mv, a->v_cache, a->head_dim, a->page_size, a->kv_heads, a->n_pages, s8[4],
+                     s8[5], s8[3]);
+  if (a->head_dim == 256) return launch_attend<256>(s.nt, boxes, mk, mv, d, s.ctas, st);
+  if (a->head_dim == 128) return launch_attend<128>(s.nt, boxes, mk, mv, d, s.ctas, st);
+  return launch_attend<64>(s.nt, boxes, mk, mv, d, s.ctas, st);
 }
 
 }  // extern "C"
