@@ -5,10 +5,14 @@
 //   y = h * rsqrt(mean(h^2) + eps) * (1 + w) | * (1 + scale) + shift | h
 //   s_g = f32(max(max_g |y|, 2^-60) / 448),  q = rne_e4m3(y / s_g)
 //
-// The codes are those of the formula without rounding in between: a value
-// computed to 32 bits lands on the wrong side of a border between two codes
-// for a few elements in a million, and is then off by a whole code, so the
-// row sum, the group maximum and the products are held in 64 bits.
+// The codes and scales are those of the formula without rounding in between:
+// a value computed to 32 bits lands on the wrong side of a border between two
+// codes for a few elements in a million, and is then off by a whole code.  All
+// of it in 64 bits is bound by the conversions (848 x 16384 bf16 codes: 24 us
+// against 6.5 us of memory traffic), so 64 bits are used where they decide:
+// the row's sum of squares, the group's largest value, and those vectors of
+// which a value, computed to 32 bits with its error bound, has a border inside
+// the bound (about one in ten thousand).
 #pragma once
 
 #include <cuda_fp8.h>
@@ -22,10 +26,15 @@ constexpr int GROUP = 128;              // columns that share a scale
 constexpr int VEC = 8;                  // columns of one thread's vector
 constexpr int LANES = GROUP / VEC;      // lanes that share a scale
 constexpr int MAX_THREADS = 512;
+// bound of the relative error of a value computed to 32 bits: 6 roundings of
+// 2^-24 and the reciprocal of the scale
+constexpr float EPS = 0x1p-20f;
 constexpr double E4M3_MAX = 448.0;
 constexpr double MIN_AMAX = 0x1p-60;
 
 enum { DELTA_NONE = 0, DELTA_F32 = 1, DELTA_BF16 = 2 };
+// what is done to a value: nothing, norm * (1 + w), norm * (1 + scale) + shift
+enum { CODES = 0, SCALE = 1, SHIFT = 2 };
 
 struct Dev {
   int mode;
@@ -42,7 +51,7 @@ struct Dev {
   float* scales;
   long long ld_scales;
   int dim;
-  double eps;
+  double eps, inv_dim;
   int vec;  // 16-byte rows everywhere: vector loads and stores
 };
 
@@ -121,10 +130,30 @@ __device__ __forceinline__ float off_border(float t, double y, double s) {
   return t;
 }
 
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+__device__ __forceinline__ float rcp(float x) {  // within an ulp
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// largest of the 16 lanes that share a scale; values not negative
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
 // One row (or, without a norm, one run of columns of a row) per CTA; thread t
 // holds VPT vectors of 8 columns, so 16 neighbouring lanes share a scale.
-template <typename TX, int DT, int VPT>
-__global__ void __launch_bounds__(MAX_THREADS) norm_fp8_kernel(const Dev p) {
+template <typename TX, int DT, int VPT, int KIND>
+__global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_kernel(const Dev p) {
+  constexpr bool NORM = KIND != CODES, ADA = KIND == SHIFT;
   __shared__ double part[MAX_THREADS / 32];
   const int T = blockDim.x, tid = threadIdx.x, lane = tid & 31;
   const long long row = blockIdx.x;
@@ -134,13 +163,16 @@ __global__ void __launch_bounds__(MAX_THREADS) norm_fp8_kernel(const Dev p) {
   griddep_wait();
   griddep_launch_dependents();
   float h[VPT][8];
-  double ss = 0.0;
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     const int c = c0 + v * T * VEC;
-    const int n = min(max(p.dim - c, 0), VEC);
-    load8(x + c, n, vec, h[v]);
-    if (DT != DELTA_NONE) {
+    load8(x + c, min(max(p.dim - c, 0), VEC), vec, h[v]);
+  }
+  if (DT != DELTA_NONE) {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int c = c0 + v * T * VEC;
+      const int n = min(max(p.dim - c, 0), VEC);
       float d[8];
       if (DT == DELTA_F32)
         load8(static_cast<const float*>(p.delta) + row * p.ld_delta + c, n, vec, d);
@@ -150,59 +182,115 @@ __global__ void __launch_bounds__(MAX_THREADS) norm_fp8_kernel(const Dev p) {
       for (int j = 0; j < 8; ++j) h[v][j] = as_stored(h[v][j] + d[j], x);
       store8(static_cast<TX*>(p.res) + row * p.ld_res + c, n, vec, h[v]);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const double e = h[v][j];
-      ss = fma(e, e, ss);
-    }
   }
   double rstd = 1.0;
-  if (p.mode != FVB_NORM_NONE) {
+  if (NORM) {
+    double ss = 0.0;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const double e = h[v][j];
+        ss = fma(e, e, ss);
+      }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if (lane == 0) part[tid >> 5] = ss;
     __syncthreads();
     ss = 0.0;
     for (int i = 0; i < T / 32; ++i) ss += part[i];
-    rstd = 1.0 / sqrt(ss / p.dim + p.eps);
+    rstd = rsqrt(fma(ss, p.inv_dim, p.eps));
   }
+  const float rf = static_cast<float>(rstd);
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     const int c = c0 + v * T * VEC;
     const int n = min(max(p.dim - c, 0), VEC);
-    double y[8];
-    if (p.mode == FVB_NORM_GEMMA_RMS) {
-      float w[8];
-      load8(p.w + c, n, vec, w);
+    // y to 32 bits, and what bounds its error: EPS * mag
+    float y[8], mag[8], w[8], b[8];
+    if (KIND == SCALE) {
+      if (p.mode == FVB_NORM_GEMMA_RMS) {
+        load8(p.w + c, n, vec, w);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = h[v][j] * rstd * (1.0 + w[j]);
-    } else if (p.mode == FVB_NORM_ADA_RMS) {
-      float s[8], b[8];
-      load8(p.mod + c, n, vec, s);
+        for (int j = 0; j < 8; ++j) w[j] = 0.f;
+      }
+    } else if (ADA) {
+      load8(p.mod + c, n, vec, w);
       load8(p.mod + p.dim + c, n, vec, b);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = h[v][j] * rstd * (1.0 + s[j]) + b[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = h[v][j] * rstd;
     }
-    double top = 0.0;  // fmax drops NaN: the others keep their codes
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = fmax(top, fabs(y[j]));
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1)
-      top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float s = static_cast<float>(fmax(top, MIN_AMAX) / E4M3_MAX);
-    const double sd = s, inv = 1.0 / sd;
-    uint32_t code[2] = {0u, 0u};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float t = off_border(static_cast<float>(y[j] * inv), y[j], sd);
-      code[j >> 2] |= static_cast<uint32_t>(
-                          __nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3))
-                      << (8 * (j & 3));
+      y[j] = NORM ? h[v][j] * rf * (1.f + w[j]) : h[v][j];
+      mag[j] = fabsf(y[j]);
+      if (ADA) {
+        mag[j] += fabsf(b[j]);
+        y[j] += b[j];
+      }
+    }
+    auto exact = [&](int j) {
+      double r = h[v][j];
+      if (NORM) r = r * rstd * (1.0 + w[j]);
+      if (ADA) r += b[j];
+      return r;
+    };
+    float s;
+    if (NORM) {
+      // of the values that may be the largest, the largest scale
+      float low = 0.f, high = 0.f;  // fmax drops NaN: the others keep their codes
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float a = fabsf(y[j]);
+        low = fmaxf(low, ADA ? fmaf(-EPS, mag[j], a) : a);
+        high = fmaxf(high, ADA ? fmaf(EPS, mag[j], a) : a);
+      }
+      if (!ADA) {
+        low *= 1.f - EPS;
+        high *= 1.f + EPS;
+      }
+      low = group_max(low);
+      s = static_cast<float>(MIN_AMAX / E4M3_MAX);
+      if (high >= low && low > 0.f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (fmaf(EPS, mag[j], fabsf(y[j])) >= low)
+            s = fmaxf(s, static_cast<float>(fabs(exact(j)) * (1.0 / E4M3_MAX)));
+      }
+      s = group_max(s);
+    } else {
+      float top = static_cast<float>(MIN_AMAX);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, mag[j]);
+      // top / 448 rounded to f32, by a multiplication and its remainder
+      // (Markstein); infinity stays infinity
+      top = group_max(top);
+      constexpr float M = static_cast<float>(E4M3_MAX), I = 1.f / M;
+      const float q = top * I;
+      s = top < INFINITY ? fmaf(fmaf(-M, q, top), I, q) : top;
     }
     if (n <= 0) continue;
+    // codes of both ends of each value's interval
+    const float r = rcp(s), r_lo = r * (1.f - EPS), r_hi = r * (1.f + EPS);
+    float lo[8], hi[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      lo[j] = ADA ? fmaf(-EPS, mag[j], y[j]) * r : y[j] * r_lo;
+      hi[j] = ADA ? fmaf(EPS, mag[j], y[j]) * r : y[j] * r_hi;
+    }
+    uint32_t code[2] = {codes4(lo[0], lo[1], lo[2], lo[3]), codes4(lo[4], lo[5], lo[6], lo[7])};
+    if (code[0] != codes4(hi[0], hi[1], hi[2], hi[3]) ||
+        code[1] != codes4(hi[4], hi[5], hi[6], hi[7])) {
+      const double sd = s, inv = 1.0 / sd;
+      code[0] = code[1] = 0u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const double e = exact(j);
+        const float t = off_border(static_cast<float>(e * inv), e, sd);
+        const uint32_t q = __nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3);
+        if (j < 4) code[0] |= q << (8 * j);
+        else code[1] |= q << (8 * j - 32);
+      }
+    }
     uint8_t* q = p.q + row * p.ld_q + c;
     if (vec && n == 8) {
       *reinterpret_cast<uint2*>(q) = make_uint2(code[0], code[1]);

@@ -46,23 +46,30 @@ int make_map_u8(CUtensorMap* m, const void* ptr, int64_t rows, int64_t k, int64_
   return FVB_OK;
 }
 
+template <typename TX, int DT, int KIND>
+int launch_norm_rows(const fvb::n8::Dev& d, int rows, cudaStream_t st) {
+  namespace N = fvb::n8;
+  const int chunks = (d.dim + N::VEC - 1) / N::VEC;
+  const int vpt = chunks <= N::MAX_THREADS ? 1 : (chunks <= 2 * N::MAX_THREADS ? 2 : 4);
+  const int t = ((chunks + vpt - 1) / vpt + 31) / 32 * 32;
+  auto kern = vpt == 1   ? N::norm_fp8_kernel<TX, DT, 1, KIND>
+              : vpt == 2 ? N::norm_fp8_kernel<TX, DT, 2, KIND>
+                         : N::norm_fp8_kernel<TX, DT, 4, KIND>;
+  return launch_k("fvb_norm_fp8", kern, dim3(rows), dim3(t), 0, st, d);
+}
+
 template <typename TX, int DT>
 int launch_norm_fp8(const fvb::n8::Dev& d, int rows, cudaStream_t st) {
   namespace N = fvb::n8;
+  if (d.mode == FVB_NORM_ADA_RMS) return launch_norm_rows<TX, DT, N::SHIFT>(d, rows, st);
+  if (d.mode != FVB_NORM_NONE) return launch_norm_rows<TX, DT, N::SCALE>(d, rows, st);
+  // no row statistics: runs of 2048 columns, each its own CTA.  (One vector a
+  // thread: 848 x 16384 takes 14.7 us, with two 17.8, with four 22.6, whose
+  // registers leave fewer warps to cover the latencies.)
   const int chunks = (d.dim + N::VEC - 1) / N::VEC;
-  if (d.mode == FVB_NORM_NONE) {
-    // no row statistics: runs of 2048 columns, each its own CTA
-    const int t = chunks < 256 ? (chunks + 31) / 32 * 32 : 256;
-    return launch_k("fvb_norm_fp8", N::norm_fp8_kernel<TX, DT, 1>,
-                    dim3(rows, (chunks + t - 1) / t), dim3(t), 0, st, d);
-  }
-  const int vpt = chunks <= N::MAX_THREADS ? 1 : (chunks <= 2 * N::MAX_THREADS ? 2 : 4);
-  const int t = ((chunks + vpt - 1) / vpt + 31) / 32 * 32;
-  if (vpt == 1)
-    return launch_k("fvb_norm_fp8", N::norm_fp8_kernel<TX, DT, 1>, dim3(rows), dim3(t), 0, st, d);
-  if (vpt == 2)
-    return launch_k("fvb_norm_fp8", N::norm_fp8_kernel<TX, DT, 2>, dim3(rows), dim3(t), 0, st, d);
-  return launch_k("fvb_norm_fp8", N::norm_fp8_kernel<TX, DT, 4>, dim3(rows), dim3(t), 0, st, d);
+  const int t = chunks < 256 ? (chunks + 31) / 32 * 32 : 256;
+  return launch_k("fvb_norm_fp8", N::norm_fp8_kernel<TX, DT, 1, N::CODES>,
+                  dim3(rows, (chunks + t - 1) / t), dim3(t), 0, st, d);
 }
 
 template <typename TX>
@@ -252,7 +259,7 @@ int fvb_norm_fp8(const fvb_norm_fp8_args* a, void* stream) {
   d.w = (const bf16*)a->w; d.mod = a->mod;
   d.q = (uint8_t*)a->q; d.ld_q = a->ld_q;
   d.scales = a->scales; d.ld_scales = a->ld_scales;
-  d.dim = a->dim; d.eps = a->eps;
+  d.dim = a->dim; d.eps = a->eps; d.inv_dim = 1.0 / a->dim;
   d.vec = rows16(a->x, a->ld_x, xb) && aligned(a->q, 8) && a->ld_q % 8 == 0 &&
           (!a->delta || (rows16(a->delta, a->ld_delta, db) && rows16(a->res, a->ld_res, xb))) &&
           (a->mode != FVB_NORM_GEMMA_RMS || aligned16(a->w)) &&
