@@ -130,6 +130,30 @@ __device__ __forceinline__ float off_border(float t, double y, double s) {
   return t;
 }
 
+// The same for a value y that f32 holds: t = |y| / s within 2^-21.  A border
+// that near is decided by y - border * s, whose sign one rounding keeps.  bf16
+// values meet borders exactly in every group whose largest value is a multiple
+// of 7, so this path has no 64-bit arithmetic.
+__device__ __forceinline__ float off_border(float t, float y, float s) {
+  const uint32_t b = __float_as_uint(t);
+  float border;
+  bool close;
+  if (b >= 0x3c7ffff0u) {  // 2^-6, less the bound
+    border = __uint_as_float((b & 0xfff00000u) | 0x80000u);
+    close = (b & 0xfffffu) - 0x7fff0u <= 0x20u;
+  } else {
+    const float r = t * 1024.f, odd = 2.f * floorf(0.5f * r) + 1.f;
+    border = odd * 0x1p-10f;
+    close = fabsf(r - odd) <= r * 0x1p-20f;
+  }
+  if (close) {
+    const float d = fmaf(-border, s, y);
+    const uint32_t c = __float_as_uint(border);
+    t = __uint_as_float(d > 0.f ? c + 1 : (d < 0.f ? c - 1 : c));
+  }
+  return t;
+}
+
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
@@ -280,16 +304,20 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
     uint32_t code[2] = {codes4(lo[0], lo[1], lo[2], lo[3]), codes4(lo[4], lo[5], lo[6], lo[7])};
     if (code[0] != codes4(hi[0], hi[1], hi[2], hi[3]) ||
         code[1] != codes4(hi[4], hi[5], hi[6], hi[7])) {
-      const double sd = s, inv = 1.0 / sd;
-      code[0] = code[1] = 0u;
+      float t[8];
+      if (NORM) {
+        const double sd = s, inv = 1.0 / sd;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const double e = exact(j);
-        const float t = off_border(static_cast<float>(e * inv), e, sd);
-        const uint32_t q = __nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3);
-        if (j < 4) code[0] |= q << (8 * j);
-        else code[1] |= q << (8 * j - 32);
+        for (int j = 0; j < 8; ++j) {
+          const double e = exact(j);
+          t[j] = off_border(static_cast<float>(e * inv), e, sd);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = copysignf(off_border(mag[j] * r, mag[j], s), y[j]);
       }
+      code[0] = codes4(t[0], t[1], t[2], t[3]);
+      code[1] = codes4(t[4], t[5], t[6], t[7]);
     }
     uint8_t* q = p.q + row * p.ld_q + c;
     if (vec && n == 8) {

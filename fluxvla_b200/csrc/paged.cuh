@@ -31,21 +31,9 @@ struct AppendDev {
   const float* rope_cs;
   int tokens, heads, kv_heads, dim;
   int page_size, max_pos, interleaved;
+  int heads_per_thread;  // VEC
   long long n_slots;
 };
-
-// 8 rotary pairs of one head: the pairs' first halves in a, second in b
-__device__ __forceinline__ void rotate8(float (&a)[8], float (&b)[8], const float* cs) {
-#pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const float4 t = __ldg(reinterpret_cast<const float4*>(cs + 2 * i));
-    const float a0 = a[i], b0 = b[i], a1 = a[i + 1], b1 = b[i + 1];
-    a[i] = a0 * t.x - b0 * t.y;
-    b[i] = b0 * t.x + a0 * t.y;
-    a[i + 1] = a1 * t.z - b1 * t.w;
-    b[i + 1] = b1 * t.z + a1 * t.w;
-  }
-}
 
 __device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
   const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
@@ -60,94 +48,157 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
                     pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
+__device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
+  const float x = a, y = b;
+  a = x * c - y * s;
+  b = y * c + x * s;
+}
 
-// One thread moves 16 elements of one head of one token (8 rotary pairs) with
-// 16-byte accesses (VEC), or 2 elements (one pair) where alignment or the
-// head size rule those out.
-template <bool VEC>
+// Where one head's row of a token comes from and goes to; false if nowhere.
+struct Row {
+  const bf16* src;
+  bf16* dst;
+};
+__device__ __forceinline__ bool row_of(const AppendDev& p, long long tok, int head, int slot,
+                                       Row* r) {
+  if (head < p.heads) {
+    r->src = p.q + tok * p.q_rs + head * p.q_hs;
+    r->dst = p.q_out + tok * p.qo_rs + head * p.qo_hs;
+    return true;
+  }
+  if (slot < 0) return false;  // a row that is not cached
+  const int page = slot / p.page_size, at = slot - page * p.page_size;
+  int h = head - p.heads;
+  if (h < p.kv_heads) {
+    r->src = p.k + tok * p.k_rs + h * p.k_hs;
+    r->dst = p.k_cache + page * p.kc_ps + at * p.kc_rs + h * p.kc_hs;
+  } else {
+    h -= p.kv_heads;
+    r->src = p.v + tok * p.v_rs + h * p.v_hs;
+    r->dst = p.v_cache + page * p.vc_ps + at * p.vc_rs + h * p.vc_hs;
+  }
+  return true;
+}
+
+// A token's slot and position; false if its rows are left alone.
+__device__ __forceinline__ bool token_of(const AppendDev& p, long long tok, int* slot, int* pos) {
+  *slot = __ldg(p.slots + tok);
+  *pos = 0;
+  bool ok = *slot < p.n_slots;
+  if (p.rope_cs) {
+    *pos = __ldg(p.positions + tok);
+    if (*pos < 0 || *pos >= p.max_pos) {
+      if (*slot < 0) return false;  // padding has no position; a cached row needs one
+      ok = false;
+    }
+  }
+  if (!ok) record_device_error(FVB_ERR_INVALID_ARG);
+  return ok;
+}
+
+// Bound by HBM: a thread moves 16 elements (8 rotary pairs, one chunk) of
+// heads_per_thread heads of one token with 16-byte accesses, four heads in
+// flight, and reads the chunk's cosines and sines once for them (a thread per
+// head read them from L1 for every head: 13056 x 10 heads of 256 took 38 us).
+__global__ void __launch_bounds__(256) append_vec_kernel(const AppendDev p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const unsigned per_head = p.dim / 16, total = p.heads + 2 * p.kv_heads;
+  const unsigned blocks = (total + p.heads_per_thread - 1) / p.heads_per_thread;
+  const unsigned per_token = per_head * blocks;
+  const long long idx = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const long long tok = idx / per_token;
+  if (tok >= p.tokens) return;
+  const unsigned item = (unsigned)(idx - tok * per_token);
+  const int blk = item / per_head, ch = item - blk * per_head;
+  const int h0 = blk * p.heads_per_thread;
+  const int h1 = min(h0 + p.heads_per_thread, (int)total);
+  const int rotated = p.rope_cs ? p.heads + p.kv_heads : 0;
+  int slot, pos;
+  if (!token_of(p, tok, &slot, &pos)) return;
+  float4 cs[4];
+  if (h0 < rotated) {
+    const float4* t = reinterpret_cast<const float4*>(p.rope_cs + ((long long)pos * (p.dim / 2) + ch * 8) * 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cs[i] = __ldg(t + i);
+  }
+  constexpr int U = 4;
+  for (int hb = h0; hb < h1; hb += U) {
+    Row row[U];
+    uint4 u[U][2];
+    bool in[U];
+    int first[U], second[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      // the two halves of the pairs: dims i and i + dim/2, or 2i and 2i + 1
+      const bool half = hb + i < rotated && !p.interleaved;
+      first[i] = ch * (half ? 8 : 16);
+      second[i] = first[i] + (half ? p.dim / 2 : 8);
+      in[i] = hb + i < h1 && row_of(p, tok, hb + i, slot, &row[i]);
+      if (in[i]) {
+        u[i][0] = *reinterpret_cast<const uint4*>(row[i].src + first[i]);
+        u[i][1] = *reinterpret_cast<const uint4*>(row[i].src + second[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (!in[i]) continue;
+      if (hb + i < rotated) {
+        float x[8], y[8];
+        unpack8(u[i][0], x);
+        unpack8(u[i][1], y);
+        if (p.interleaved) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            rotate(x[4 * j], x[4 * j + 1], cs[j].x, cs[j].y);
+            rotate(x[4 * j + 2], x[4 * j + 3], cs[j].z, cs[j].w);
+            rotate(y[4 * j], y[4 * j + 1], cs[2 + j].x, cs[2 + j].y);
+            rotate(y[4 * j + 2], y[4 * j + 3], cs[2 + j].z, cs[2 + j].w);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            rotate(x[2 * j], y[2 * j], cs[j].x, cs[j].y);
+            rotate(x[2 * j + 1], y[2 * j + 1], cs[j].z, cs[j].w);
+          }
+        }
+        u[i][0] = pack8(x);
+        u[i][1] = pack8(y);
+      }
+      *reinterpret_cast<uint4*>(row[i].dst + first[i]) = u[i][0];
+      *reinterpret_cast<uint4*>(row[i].dst + second[i]) = u[i][1];
+    }
+  }
+}
+
+// One rotary pair of one head a thread, where alignment or the head size rule
+// 16-byte accesses out.
 __global__ void __launch_bounds__(256) append_kernel(const AppendDev p) {
   griddep_wait();
   griddep_launch_dependents();
-  constexpr int EL = VEC ? 16 : 2;
-  const unsigned per_head = p.dim / EL;
+  const unsigned per_head = p.dim / 2;
   const unsigned per_token = per_head * (p.heads + 2 * p.kv_heads);
   const long long idx = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   const long long tok = idx / per_token;
   if (tok >= p.tokens) return;
   const unsigned item = (unsigned)(idx - tok * per_token);
   const int head = item / per_head, ch = item - head * per_head;
-  const int slot = __ldg(p.slots + tok);
-  const bool is_q = head < p.heads, is_v = head >= p.heads + p.kv_heads;
-  if (slot < 0 && !is_q) return;  // a row that is not cached
-  int pos = 0;
-  if (p.rope_cs) {
-    pos = __ldg(p.positions + tok);
-    if (pos < 0 || pos >= p.max_pos) {
-      // padding has no position; a cached row needs one
-      if (slot >= 0) record_device_error(FVB_ERR_INVALID_ARG);
-      return;
-    }
+  int slot, pos;
+  Row row;
+  if (!token_of(p, tok, &slot, &pos) || !row_of(p, tok, head, slot, &row)) return;
+  const bool turn = p.rope_cs && head < p.heads + p.kv_heads;
+  const bool half = turn && !p.interleaved;
+  const int first = half ? ch : 2 * ch, second = half ? ch + p.dim / 2 : 2 * ch + 1;
+  bf16 a = row.src[first], b = row.src[second];
+  if (turn) {
+    const float2 cs = __ldg(reinterpret_cast<const float2*>(p.rope_cs) + (long long)pos * per_head + ch);
+    float x = __bfloat162float(a), y = __bfloat162float(b);
+    rotate(x, y, cs.x, cs.y);
+    a = __float2bfloat16(x);
+    b = __float2bfloat16(y);
   }
-  if (slot >= p.n_slots) {
-    record_device_error(FVB_ERR_INVALID_ARG);
-    return;
-  }
-  const bf16* src;
-  bf16* dst;
-  if (is_q) {
-    src = p.q + tok * p.q_rs + head * p.q_hs;
-    dst = p.q_out + tok * p.qo_rs + head * p.qo_hs;
-  } else {
-    const int page = slot / p.page_size, at = slot - page * p.page_size;
-    const int h = head - p.heads - (is_v ? p.kv_heads : 0);
-    src = is_v ? p.v + tok * p.v_rs + h * p.v_hs : p.k + tok * p.k_rs + h * p.k_hs;
-    dst = is_v ? p.v_cache + page * p.vc_ps + at * p.vc_rs + h * p.vc_hs
-               : p.k_cache + page * p.kc_ps + at * p.kc_rs + h * p.kc_hs;
-  }
-  const bool turn = !is_v && p.rope_cs;
-  const float* cs = turn ? p.rope_cs + ((long long)pos * (p.dim / 2) + ch * (EL / 2)) * 2 : nullptr;
-  // the two halves of the pairs: dims i and i + dim/2, or 2i and 2i + 1
-  const int first = turn && !p.interleaved ? ch * (EL / 2) : ch * EL;
-  const int second = turn && !p.interleaved ? first + p.dim / 2 : first + EL / 2;
-  if (VEC) {
-    uint4 u0 = *reinterpret_cast<const uint4*>(src + first);
-    uint4 u1 = *reinterpret_cast<const uint4*>(src + second);
-    if (turn) {
-      float x[8], y[8];
-      unpack8(u0, x);
-      unpack8(u1, y);
-      if (p.interleaved) {
-        float a[8], b[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          a[i] = x[2 * i]; b[i] = x[2 * i + 1];
-          a[4 + i] = y[2 * i]; b[4 + i] = y[2 * i + 1];
-        }
-        rotate8(a, b, cs);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[2 * i] = a[i]; x[2 * i + 1] = b[i];
-          y[2 * i] = a[4 + i]; y[2 * i + 1] = b[4 + i];
-        }
-      } else {
-        rotate8(x, y, cs);
-      }
-      u0 = pack8(x);
-      u1 = pack8(y);
-    }
-    *reinterpret_cast<uint4*>(dst + first) = u0;
-    *reinterpret_cast<uint4*>(dst + second) = u1;
-  } else {
-    bf16 a = src[first], b = src[second];
-    if (turn) {
-      const float fa = __bfloat162float(a), fb = __bfloat162float(b);
-      const float c = __ldg(cs), s = __ldg(cs + 1);
-      a = __float2bfloat16(fa * c - fb * s);
-      b = __float2bfloat16(fb * c + fa * s);
-    }
-    dst[first] = a;
-    dst[second] = b;
-  }
+  row.dst[first] = a;
+  row.dst[second] = b;
 }
 
 // ---------------------------------------------------------------------------

@@ -379,13 +379,19 @@ int fvb_paged_append(const fvb_paged_append_args* a, void* stream) {
                              d.kc_ps, d.kc_rs, d.kc_hs, d.vc_ps, d.vc_rs, d.vc_hs};
   for (int i = a->heads > 0 ? 0 : 2; i < 14; ++i)
     if (a->heads > 0 || (i != 6 && i != 7)) vec = vec && strides[i] % 8 == 0;
-  const int64_t per_token = (int64_t)(a->heads + 2 * a->kv_heads) * (a->head_dim / (vec ? 16 : 2));
+  // all heads of a token in one thread where the tokens fill the GPU by
+  // themselves, else a head each
+  const int64_t heads = (int64_t)a->heads + 2ll * a->kv_heads;
+  const int64_t chunks = a->head_dim / (vec ? 16 : 2);
+  const bool many = chunks * a->tokens >= 256ll * 2 * sm_count();
+  d.heads_per_thread = many && heads < INT32_MAX ? (int)heads : 1;
+  const int64_t per_token = vec && many ? chunks : heads * chunks;
   const int64_t blocks = (per_token * a->tokens + 255) / 256;
-  if (per_token > INT32_MAX || blocks > INT32_MAX)
+  if (heads * chunks > INT32_MAX || blocks > INT32_MAX)
     return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_append: too many rows");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return launch_k("fvb_paged_append",
-                  vec ? fvb::paged::append_kernel<true> : fvb::paged::append_kernel<false>,
+                  vec ? fvb::paged::append_vec_kernel : fvb::paged::append_kernel,
                   dim3((unsigned)blocks), dim3(256), 0, st, d);
 }
 
