@@ -425,6 +425,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t ring = smem_u32(ring_ptr);
   if (lane == 0)
     for (int s = 0; s < C::SLOTS; ++s) mbar_init(&full[s], 1);
+  if (BOXES && tid == 0) {
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
+  }
   fence_barrier_init();
   griddep_wait();
   griddep_launch_dependents();
@@ -608,9 +612,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   };
   start_pages();
-  load_q();
 #pragma unroll 1
   for (int i = 0; i < C::SLOTS; ++i) request();
+  load_q();
 
   bool alive = true;
   while (true) {
@@ -740,9 +744,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       run = locate(u);
       requested = 0;
       start_pages();
-      load_q();
 #pragma unroll 1
       for (int i = 0; i < C::SLOTS - NT; ++i) request();
+      load_q();
     }
     // join the warps: factors from the common maximum, then the sum of O
 #pragma unroll
