@@ -226,6 +226,9 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
     rstd = rsqrt(fma(ss, p.inv_dim, p.eps));
   }
   const float rf = static_cast<float>(rstd);
+  // near the ends of the 32-bit range the bounds do not hold (nor where rf is
+  // NaN): such rows are computed in 64 bits throughout
+  const bool fine = !NORM || (rf >= 0x1p-100f && rf <= 0x1p100f);
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     const int c = c0 + v * T * VEC;
@@ -274,10 +277,10 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
       }
       low = group_max(low);
       s = static_cast<float>(MIN_AMAX / E4M3_MAX);
-      if (high >= low && low > 0.f) {
+      if (!fine || (high >= low && low > 0.f)) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (fmaf(EPS, mag[j], fabsf(y[j])) >= low)
+          if (!fine || fmaf(EPS, mag[j], fabsf(y[j])) >= low)
             s = fmaxf(s, static_cast<float>(fabs(exact(j)) * (1.0 / E4M3_MAX)));
       }
       s = group_max(s);
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
       hi[j] = ADA ? fmaf(EPS, mag[j], y[j]) * r : y[j] * r_hi;
     }
     uint32_t code[2] = {codes4(lo[0], lo[1], lo[2], lo[3]), codes4(lo[4], lo[5], lo[6], lo[7])};
-    if (code[0] != codes4(hi[0], hi[1], hi[2], hi[3]) ||
+    if (!fine || code[0] != codes4(hi[0], hi[1], hi[2], hi[3]) ||
         code[1] != codes4(hi[4], hi[5], hi[6], hi[7])) {
       float t[8];
       if (NORM) {

@@ -11,8 +11,14 @@
 using namespace fvb_host;
 
 // This translation unit's status word (common.cuh), read and reset through
-// fvb_get_device_status.
+// fvb_get_device_status once one of its kernels has been launched.
+static std::atomic<bool> g_used{false};
+
 int fvb_serving_device_status(int* status, int reset) {
+  if (!g_used.load(std::memory_order_relaxed)) {
+    *status = FVB_OK;
+    return FVB_OK;
+  }
   cudaError_t e = cudaMemcpyFromSymbol(status, g_fvb_device_status, sizeof(int));
   if (e == cudaSuccess && reset) {
     const int z = 0;
@@ -249,6 +255,7 @@ int fvb_norm_fp8(const fvb_norm_fp8_args* a, void* stream) {
     return fail(FVB_ERR_INVALID_ARG, "fvb_norm_fp8: a row stride is shorter than its row");
   if (!(a->eps >= 0)) return fail(FVB_ERR_INVALID_ARG, "fvb_norm_fp8: bad eps");
   if (a->rows == 0) return FVB_OK;
+  g_used.store(true, std::memory_order_relaxed);
   const int xb = a->x_f32 ? 4 : 2, db = a->delta_f32 ? 4 : 2;
   auto rows16 = [](const void* p, int64_t ld, int eb) { return aligned16(p) && ld * eb % 16 == 0; };
   fvb::n8::Dev d;
@@ -290,6 +297,7 @@ int fvb_gemm_fp8(const fvb_gemm_fp8_args* a, void* stream) {
     return fail(FVB_ERR_INVALID_ARG,
                 "fvb_gemm_fp8: operands must be 16B aligned with row strides in multiples of 16");
   if (a->m == 0) return FVB_OK;
+  g_used.store(true, std::memory_order_relaxed);
   fvb::g8::Dev d;
   d.m = a->m; d.n = a->n; d.groups = groups;
   d.sa = a->a_scale; d.ld_sa = a->ld_as;
@@ -360,6 +368,7 @@ int fvb_paged_append(const fvb_paged_append_args* a, void* stream) {
   if (a->rope_cs && (!a->positions || a->max_pos <= 0 || !aligned(a->rope_cs, 8)))
     return fail(FVB_ERR_INVALID_ARG, "fvb_paged_append: rope_cs needs positions and max_pos");
   if (a->tokens == 0) return FVB_OK;
+  g_used.store(true, std::memory_order_relaxed);
   fvb::paged::AppendDev d;
   d.q = (const bf16*)a->q; d.q_rs = a->q_row_stride; d.q_hs = a->q_head_stride;
   d.k = (const bf16*)a->k; d.k_rs = a->k_row_stride; d.k_hs = a->k_head_stride;
@@ -432,6 +441,7 @@ int fvb_paged_attention(const fvb_paged_attn_args* a, void* stream) {
     return fail(FVB_ERR_WORKSPACE, "fvb_paged_attention: workspace needs %lld bytes",
                 (long long)s.bytes);
   if (a->batch == 0) return FVB_OK;
+  g_used.store(true, std::memory_order_relaxed);
   fvb::paged::AttendDev d;
   d.q = (const bf16*)a->q; d.q_rs = a->q_row_stride; d.q_hs = a->q_head_stride;
   d.k = (const bf16*)a->k_cache; d.k_ps = s8[0]; d.k_rs = s8[1]; d.k_hs = s8[2];

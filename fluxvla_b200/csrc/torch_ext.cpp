@@ -176,6 +176,9 @@ int64_t strided(const at::Tensor& t, at::ScalarType dt, int64_t dims, const char
   return dims == 2 && t.size(0) <= 1 ? std::max(t.stride(0), t.size(1)) : t.stride(0);
 }
 
+// stride of a dimension; one of size 1 has none that matters
+int64_t step(const at::Tensor& t, int64_t dim) { return t.size(dim) <= 1 ? 0 : t.stride(dim); }
+
 void same_device(const at::Tensor& a, const at::Tensor& b, const char* name) {
   require(a.device() == b.device(), name, ": on ", b.device(), ", expected ", a.device());
 }
@@ -285,9 +288,9 @@ void gemm_fp8(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& 
 void cache_strides(const at::Tensor& c, const char* name, int64_t* page, int64_t* row,
                    int64_t* head) {
   strided(c, at::kBFloat16, 4, name);
-  *page = c.stride(0);
-  *row = c.stride(1);
-  *head = c.stride(2);
+  *page = step(c, 0);
+  *row = step(c, 1);
+  *head = step(c, 2);
 }
 
 int32_t* int_vector(const at::Tensor& t, int64_t n, const char* name) {
@@ -302,10 +305,12 @@ void paged_append(const OptT& q, const at::Tensor& k, const at::Tensor& v,
                   bool rope_interleaved) {
   fvb_paged_append_args a;
   memset(&a, 0, sizeof(a));
-  a.k_row_stride = strided(k, at::kBFloat16, 3, "k");
-  a.v_row_stride = strided(v, at::kBFloat16, 3, "v");
-  a.k_head_stride = k.stride(1);
-  a.v_head_stride = v.stride(1);
+  strided(k, at::kBFloat16, 3, "k");
+  strided(v, at::kBFloat16, 3, "v");
+  a.k_row_stride = step(k, 0);
+  a.v_row_stride = step(v, 0);
+  a.k_head_stride = step(k, 1);
+  a.v_head_stride = step(v, 1);
   a.tokens = i32(k.size(0), "tokens");
   a.kv_heads = i32(k.size(1), "kv_heads");
   a.head_dim = i32(k.size(2), "head_dim");
@@ -322,10 +327,12 @@ void paged_append(const OptT& q, const at::Tensor& k, const at::Tensor& v,
   for (const at::Tensor* t : {&v, &slots, &k_cache, &v_cache}) same_device(k, *t, "operand");
   require(q.has_value() == q_out.has_value(), "q and q_out come together");
   if (q.has_value()) {
-    a.q_row_stride = strided(*q, at::kBFloat16, 3, "q");
-    a.q_out_row_stride = strided(*q_out, at::kBFloat16, 3, "q_out");
-    a.q_head_stride = q->stride(1);
-    a.q_out_head_stride = q_out->stride(1);
+    strided(*q, at::kBFloat16, 3, "q");
+    strided(*q_out, at::kBFloat16, 3, "q_out");
+    a.q_row_stride = step(*q, 0);
+    a.q_out_row_stride = step(*q_out, 0);
+    a.q_head_stride = step(*q, 1);
+    a.q_out_head_stride = step(*q_out, 1);
     a.heads = i32(q->size(1), "heads");
     require(q->size(0) == a.tokens && q->size(2) == a.head_dim && q_out->sizes() == q->sizes(),
             "q and q_out: expected [", a.tokens, ", heads, ", a.head_dim, "], got ", q->sizes(),
@@ -363,10 +370,12 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::T
                      const at::Tensor& workspace) {
   fvb_paged_attn_args a;
   memset(&a, 0, sizeof(a));
-  a.q_row_stride = strided(q, at::kBFloat16, 3, "q");
-  a.out_row_stride = strided(out, at::kBFloat16, 3, "out");
-  a.q_head_stride = q.stride(1);
-  a.out_head_stride = out.stride(1);
+  strided(q, at::kBFloat16, 3, "q");
+  strided(out, at::kBFloat16, 3, "out");
+  a.q_row_stride = step(q, 0);
+  a.out_row_stride = step(out, 0);
+  a.q_head_stride = step(q, 1);
+  a.out_head_stride = step(out, 1);
   require(out.sizes() == q.sizes(), "out: expected ", q.sizes(), ", got ", out.sizes());
   a.batch = i32(q.size(0), "batch");
   a.heads = i32(q.size(1), "heads");

@@ -440,8 +440,9 @@ typedef struct fvb_paged_attn_args {
  * page 0, and either sets FVB_ERR_INVALID_ARG in the device status word.
  *
  * The workspace must be zero-filled before its first use and every call
- * leaves it ready for the next, of any shape.  Calls that share one must not
- * overlap on the GPU.  The partial sums of a sequence are joined in the order
+ * leaves it ready for the next, of any shape (after FVB_ERR_DEVICE_TIMEOUT it
+ * must be zero-filled again).  Calls that share one must not overlap on the
+ * GPU.  The partial sums of a sequence are joined in the order
  * of its keys: the same call gives the same bits.                           */
 int fvb_paged_attention(const fvb_paged_attn_args* args, void* stream);
 /* Workspace bytes for this head_dim, heads and kv_heads on the current

@@ -140,6 +140,38 @@ def test_norm_fp8_zero_tiny_nan_and_infinite_rows():
     assert (values(q[:1]) == 0).all()
 
 
+@pytest.mark.parametrize('mode', ['gemma', 'ada', 'rms'])
+@pytest.mark.parametrize('size,eps', [(1e38, 1e-6), (1e-18, 1e-6), (1e-30, 0.0),
+                                      (3e-39, 0.0), (1e30, 0.0)])
+def test_norm_fp8_at_the_ends_of_the_range(mode, size, eps):
+    """Rows whose norm factor 32 bits hold badly or not at all."""
+    g = gen(9)
+    x, kw = norm_inputs(g, 4, 300, mode, F32, None)
+    x = (x.double() / x.abs().max() * size).float()
+    q = torch.empty(4, 300, dtype=E4M3, device=DEV)
+    s = torch.empty(4, 3, device=DEV)
+    ops.norm_fp8(MODES[mode], x, q, s, eps=eps, **kw)
+    _, q_ref, s_ref = R.norm_fp8(MODES[mode], x, eps=eps, **kw)
+    assert torch.equal(s, s_ref) and torch.equal(values(q), q_ref)
+
+
+@pytest.mark.parametrize('dt', [F32, BF16])
+def test_norm_fp8_many_codes(dt):
+    """Over a million values, and groups whose largest value is a multiple of 7:
+    scales that make values meet borders exactly."""
+    g = gen(10)
+    x = randn(g, 1024, 1024, dt=dt)
+    big = torch.tensor([3.5, 7.0, 8.75, 14.0], device=DEV)
+    x[:512, ::128] = big[torch.arange(512, device=DEV) % 4, None].to(dt)
+    q = torch.empty(1024, 1024, dtype=E4M3, device=DEV)
+    s = torch.empty(1024, 8, device=DEV)
+    ops.norm_fp8(_lib.NORM_NONE, x, q, s)
+    check_norm('none', x, {}, q, s)
+    w = randn(g, 1024, dt=BF16) * 0.1
+    ops.norm_fp8(_lib.NORM_GEMMA_RMS, x, q, s, w=w)
+    check_norm('gemma', x, dict(w=w), q, s)
+
+
 # ---------------------------------------------------------------- gemm_fp8
 def gemm_inputs(g, m, n, k):
     x = randn(g, m, k)
@@ -180,7 +212,8 @@ EPIS = {'bf16': _lib.EPI_BF16, 'f32': _lib.EPI_F32_STORE,
     (1, 2, 1), (1, 128, 128), (1, 2560, 2048), (3, 130, 144), (16, 256, 300),
     (17, 1152, 4304), (33, 254, 1000), (51, 1024, 4096), (64, 2048, 16384),
     (65, 128, 256), (100, 514, 640), (128, 256, 128), (129, 130, 272),
-    (300, 1152, 1152), (816, 2560, 2048), (257, 4098, 1040)])
+    (300, 1152, 1152), (816, 2560, 2048), (257, 4098, 1040),
+    (1500, 4100, 272), (2049, 8194, 1000), (8, 384, 5000), (4000, 2, 16)])
 def test_gemm_fp8(epi, m, n, k):
     g = gen(m + 3 * n + 7 * k)
     kp = -(-k // 16) * 16          # rows of 16-byte multiples
@@ -424,6 +457,64 @@ def test_paged_attention_views_large_scores_and_no_lse():
     assert torch.equal(out, out2)
     check_attention(out2, lse, q, kc, vc, table, ln, scale)
     assert (outw[:, :2] == 9).all() and (outw[:, 6:] == 9).all()
+
+
+def test_single_rows_heads_and_pages_of_any_stride():
+    """A dimension of size 1 has no stride that could be misaligned."""
+    g = gen(16)
+    pool = randn(g, 64 * 16 + 7, dt=BF16)
+    kc = pool[:1024].as_strided((1, 16, 1, 64), (3, 64, 5, 1))
+    vc = pool[:1024].as_strided((1, 16, 1, 64), (1, 64, 7, 1))
+    q = randn(g, 64, dt=BF16).as_strided((1, 1, 64), (13, 11, 1))
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    ln = torch.tensor([13], dtype=torch.int32, device=DEV)
+    out = torch.empty(64, dtype=BF16, device=DEV).as_strided((1, 1, 64), (3, 1, 1))
+    lse = torch.empty(1, 1, device=DEV)
+    ops.paged_attention(q, kc, vc, table, ln, out, scale=0.2, lse=lse,
+                        workspace=workspace(1, 1, 64))
+    check_attention(out, lse, q, kc, vc, table, ln, 0.2)
+    # one kv head seen as four (a stride of 0): read row by row
+    kc4, vc4 = kc.expand(1, 16, 4, 64), vc.expand(1, 16, 4, 64)
+    q4 = randn(g, 1, 8, 64, dt=BF16)
+    out, lse = torch.empty_like(q4), torch.empty(1, 8, device=DEV)
+    ops.paged_attention(q4, kc4, vc4, table, ln, out, scale=0.2, lse=lse,
+                        workspace=workspace(8, 4, 64))
+    check_attention(out, lse, q4, kc4, vc4, table, ln, 0.2)
+
+
+def test_calls_on_two_streams_and_graphs_that_share_a_workspace():
+    g = gen(17)
+    a = paged_inputs(g, [4000, 10, 900], 8, 1, 128, 16)
+    b = paged_inputs(g, [77] * 50, 16, 2, 64, 7)
+    outs = [torch.empty_like(a[0]), torch.empty_like(b[0])]
+    lses = [torch.empty(3, 8, device=DEV), torch.empty(50, 16, device=DEV)]
+    wss = [workspace(8, 1, 128), workspace(16, 2, 64)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, args in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                ops.paged_attention(*args, outs[i], scale=0.1, lse=lses[i],
+                                    workspace=wss[i])
+    torch.cuda.synchronize()
+    for i, args in enumerate((a, b)):
+        check_attention(outs[i], lses[i], *args, 0.1)
+    # two graphs on one workspace, replayed one after the other
+    ws = torch.zeros(max(w.numel() for w in wss), dtype=torch.uint8, device=DEV)
+    graphs = []
+    for i, args in enumerate((a, b)):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=streams[0]):
+            ops.paged_attention(*args, outs[i], scale=0.1, lse=lses[i], workspace=ws)
+    for o in outs:
+        o.fill_(5.0)
+    for _ in range(10):
+        graphs[0].replay()
+        graphs[1].replay()
+    torch.cuda.synchronize()
+    for i, args in enumerate((a, b)):
+        check_attention(outs[i], lses[i], *args, 0.1)
+    assert ops.device_status() == 0
 
 
 def test_paged_attention_bad_lengths_and_pages_are_reported():
