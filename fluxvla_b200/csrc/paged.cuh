@@ -97,9 +97,10 @@ __device__ __forceinline__ bool token_of(const AppendDev& p, long long tok, int*
 }
 
 // Bound by HBM: a thread moves 16 elements (8 rotary pairs, one chunk) of
-// heads_per_thread heads of one token with 16-byte accesses, four heads in
+// heads_per_thread heads of one token with 16-byte accesses, two heads in
 // flight, and reads the chunk's cosines and sines once for them (a thread per
-// head read them from L1 for every head: 13056 x 10 heads of 256 took 38 us).
+// head read them from L1 for every head: 13056 x 10 heads of 256 took 38 us, now
+// 25.7; four heads in flight, whose registers leave fewer threads, 28.6).
 __global__ void __launch_bounds__(256) append_vec_kernel(const AppendDev p) {
   griddep_wait();
   griddep_launch_dependents();
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(256) append_vec_kernel(const AppendDev p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) cs[i] = __ldg(t + i);
   }
-  constexpr int U = 4;
+  constexpr int U = 2;
   for (int hb = h0; hb < h1; hb += U) {
     Row row[U];
     uint4 u[U][2];
