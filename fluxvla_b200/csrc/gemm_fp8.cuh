@@ -58,7 +58,7 @@ struct Dev {
   long long ld_sb;
   void* out;
   long long ldo;
-  int vec_out;       // rows of out take 16-byte stores
+  int vec_out;       // rows of out start and end on 16 bytes, n % 8 == 0
 };
 
 // kind::f8f6f4, e4m3 x e4m3 -> f32, both K-major
@@ -182,54 +182,31 @@ __device__ __forceinline__ void geglu2(float x0, float u0, float x1, float u1, f
   y1 = x1 * u1 * (r * d0);
 }
 
-// Writes NF consecutive features f.. of token t (NF = 8; for GEGLU
-// features 2i, 2i+1 are gate and up of output i), cut at the last feature.
-template <int NF, int EPI>
-__device__ __forceinline__ void store_features(const Dev& p, int t, int f, const float (&v)[NF]) {
-  if (t >= p.m || f >= p.n) return;
-  const int nf = min(NF, p.n - f);
+// gelu(x) * up for one pair
+__device__ __forceinline__ float geglu(float x, float up) {
+  float y, unused;
+  geglu2(x, up, 0.f, 0.f, y, unused);
+  return y;
+}
+
+// Writes 8 consecutive features f.. of token t (for GEGLU features 2i, 2i+1
+// are gate and up of output i) to rows that take 16-byte stores.
+template <int EPI>
+__device__ __forceinline__ void store8(const Dev& p, int t, int f, const float (&v)[8]) {
   if (EPI == FVB_EPI_F32_STORE) {
     float* o = static_cast<float*>(p.out) + (long long)t * p.ldo + f;
-    if (p.vec_out && nf == NF) {
-#pragma unroll
-      for (int j = 0; j < NF; j += 4)
-        *reinterpret_cast<float4*>(o + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < NF; ++j)
-        if (j < nf) o[j] = v[j];
-    }
-    return;
-  }
-  constexpr int NO = EPI == FVB_EPI_GEGLU ? NF / 2 : NF;
-  const int no = EPI == FVB_EPI_GEGLU ? nf / 2 : nf;
-  float y[NO];
-#pragma unroll
-  for (int j = 0; j < NO; j += 2) {
-    if (EPI == FVB_EPI_GEGLU) {
-      geglu2(v[2 * j % NF], v[(2 * j + 1) % NF], v[(2 * j + 2) % NF], v[(2 * j + 3) % NF], y[j],
-             y[j + 1]);
-    } else {
-      y[j] = v[j];
-      y[j + 1] = v[j + 1];
-    }
-  }
-  bf16* o = static_cast<bf16*>(p.out) + (long long)t * p.ldo + (EPI == FVB_EPI_GEGLU ? f >> 1 : f);
-  if (p.vec_out && no == NO) {
-    uint32_t w[NO / 2];
-#pragma unroll
-    for (int j = 0; j < NO; j += 2) w[j / 2] = pack_bf16x2(y[j], y[j + 1]);
-    if (NO == 8)
-      *reinterpret_cast<uint4*>(o) =
-          make_uint4(w[0], w[1 % (NO / 2)], w[2 % (NO / 2)], w[3 % (NO / 2)]);
-    else if (NO == 4)
-      *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1 % (NO / 2)]);
-    else
-      *reinterpret_cast<uint32_t*>(o) = w[0];
+    *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(o + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else if (EPI == FVB_EPI_BF16) {
+    *reinterpret_cast<uint4*>(static_cast<bf16*>(p.out) + (long long)t * p.ldo + f) =
+        make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                   pack_bf16x2(v[6], v[7]));
   } else {
-#pragma unroll
-    for (int j = 0; j < NO; ++j)
-      if (j < no) o[j] = __float2bfloat16(y[j]);
+    float y[4];
+    geglu2(v[0], v[1], v[2], v[3], y[0], y[1]);
+    geglu2(v[4], v[5], v[6], v[7], y[2], y[3]);
+    *reinterpret_cast<uint2*>(static_cast<bf16*>(p.out) + (long long)t * p.ldo + (f >> 1)) =
+        make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
   }
 }
 
@@ -480,24 +457,43 @@ __global__ void __launch_bounds__(THREADS, 1)
   // this CTA's tokens: the cluster's partials in the order of the groups
   const float* part = reinterpret_cast<const float*>(cl > 1 ? recv : smem);
   if (cl > 1) mbar_wait_cluster(recvd, 0);
-  constexpr int NF = 8;
-#pragma unroll 2
-  for (int e = threadIdx.x; e < per * (C::TILE / NF); e += THREADS) {
-    const int r = e / (C::TILE / NF), f = e % (C::TILE / NF) * NF;
-    float v[NF];
-#pragma unroll
-    for (int j = 0; j < NF; j += 4)
-      *reinterpret_cast<float4*>(v + j) =
-          *reinterpret_cast<const float4*>(part + r * C::PITCH + f + j);
+  auto sum4 = [&](int r, int f) {
+    float4 v = *reinterpret_cast<const float4*>(part + r * C::PITCH + f);
     for (int i = 1; i < cl; ++i) {
-#pragma unroll
-      for (int j = 0; j < NF; j += 4) {
-        const float4 w =
-            *reinterpret_cast<const float4*>(part + (i * per + r) * C::PITCH + f + j);
-        v[j] += w.x; v[j + 1] += w.y; v[j + 2] += w.z; v[j + 3] += w.w;
-      }
+      const float4 w = *reinterpret_cast<const float4*>(part + (i * per + r) * C::PITCH + f);
+      v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
     }
-    store_features<NF, EPI>(p, t0 + my0 + r, f0 + f, v);
+    return v;
+  };
+  if (p.vec_out) {
+#pragma unroll 2
+    for (int e = threadIdx.x; e < per * (C::TILE / 8); e += THREADS) {
+      const int r = e / (C::TILE / 8), f = e % (C::TILE / 8) * 8;
+      const float4 a = sum4(r, f), b = sum4(r, f + 4);
+      const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      if (t0 + my0 + r < p.m && f0 + f < p.n) store8<EPI>(p, t0 + my0 + r, f0 + f, v);
+    }
+  } else {
+    // rows that are not 16-byte aligned, or end inside the tile: consecutive
+    // lanes write consecutive values
+    constexpr int W = EPI == FVB_EPI_GEGLU ? 2 : 1;  // features of a value
+#pragma unroll 4
+    for (int e = threadIdx.x; e < per * (C::TILE / W); e += THREADS) {
+      const int r = e / (C::TILE / W), f = e % (C::TILE / W) * W;
+      if (t0 + my0 + r >= p.m || f0 + f >= p.n) continue;
+      float v[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        v[j] = part[r * C::PITCH + f + j];
+        for (int i = 1; i < cl; ++i) v[j] += part[(i * per + r) * C::PITCH + f + j];
+      }
+      const long long at = (long long)(t0 + my0 + r) * p.ldo + (f0 + f) / W;
+      if (EPI == FVB_EPI_F32_STORE)
+        static_cast<float*>(p.out)[at] = v[0];
+      else
+        static_cast<bf16*>(p.out)[at] =
+            __float2bfloat16(EPI == FVB_EPI_GEGLU ? geglu(v[0], v[W - 1]) : v[0]);
+    }
   }
   if (cl > 1) {
     // the copies out of this CTA have been received everywhere
@@ -544,7 +540,10 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster)
                : "memory");
 }
-template <int EPI>
+// VEC: rows of out start and end on 16 bytes.  (A kernel of its own for the
+// others: with both in one the sums spill, 71 us become 86 on 816 x 32768 x
+// 2048.)
+template <int EPI, bool VEC>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_fp8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                   const Dev p) {
@@ -706,7 +705,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // go through shared memory (16-byte pieces swizzled by the row), so that
       // each store instruction writes 64 bytes of 8 rows.
       constexpr int FC = EPI == FVB_EPI_F32_STORE ? 16 : (EPI == FVB_EPI_BF16 ? 32 : 64);
-      const int eb = EPI == FVB_EPI_F32_STORE ? 4 : 2;
+      constexpr int eb = EPI == FVB_EPI_F32_STORE ? 4 : 2;
       const int nf_out = EPI == FVB_EPI_GEGLU ? p.n / 2 : p.n;
 #pragma unroll
       for (int c = 0; c < C::COLS; c += FC) {
@@ -732,27 +731,40 @@ __global__ void __launch_bounds__(THREADS, 1)
                        "r"(v[4 * j]), "r"(v[4 * j + 1]), "r"(v[4 * j + 2]), "r"(v[4 * j + 3])
                        : "memory");
         __syncwarp();
-        const int o0 = (EPI == FVB_EPI_GEGLU ? (f0 + c) >> 1 : f0 + c) + (lane & 3) * (16 / eb);
+        const int o0 = EPI == FVB_EPI_GEGLU ? (f0 + c) >> 1 : f0 + c;
+        if (VEC) {
+          const int col = o0 + (lane & 3) * (16 / eb);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = i * 8 + (lane >> 2);
-          uint32_t x[4];
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                       : "r"(stg + row * 64 + (((lane & 3) ^ (row >> 1)) & 3) * 16));
-          if (t0 + row >= p.m || o0 >= nf_out) continue;
-          uint8_t* o = static_cast<uint8_t*>(p.out) + ((long long)(t0 + row) * p.ldo + o0) * eb;
-          if (p.vec_out && o0 + 16 / eb <= nf_out) {
-            *reinterpret_cast<uint4*>(o) = make_uint4(x[0], x[1], x[2], x[3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16 / eb; ++j)
-              if (o0 + j < nf_out) {
-                if (eb == 4)
-                  reinterpret_cast<uint32_t*>(o)[j] = x[j & 3];
-                else
-                  reinterpret_cast<uint16_t*>(o)[j] = (uint16_t)(x[j >> 1] >> (16 * (j & 1)));
-              }
+          for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + (lane >> 2);
+            uint32_t x[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                         : "r"(stg + row * 64 + (((lane & 3) ^ (row >> 1)) & 3) * 16));
+            if (t0 + row < p.m && col < nf_out)
+              *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) +
+                                        ((long long)(t0 + row) * p.ldo + col) * eb) =
+                  make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        } else {
+          // consecutive lanes write consecutive values
+          constexpr int PER = EPI == FVB_EPI_F32_STORE ? 16 : 32;  // values of a row
+          const int col = lane % PER;
+#pragma unroll 2
+          for (int i = 0; i < PER; ++i) {
+            const int row = i * (32 / PER) + lane / PER, at = col * eb;
+            const uint32_t src = stg + row * 64 + (((at >> 4) ^ (row >> 1)) & 3) * 16 + (at & 15);
+            if (t0 + row >= p.m || o0 + col >= nf_out) continue;
+            const long long to = (long long)(t0 + row) * p.ldo + o0 + col;
+            if (EPI == FVB_EPI_F32_STORE) {
+              uint32_t x;
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(src));
+              static_cast<uint32_t*>(p.out)[to] = x;
+            } else {
+              uint16_t x;
+              asm volatile("ld.shared.b16 %0, [%1];" : "=h"(x) : "r"(src));
+              static_cast<uint16_t*>(p.out)[to] = x;
+            }
           }
         }
       }

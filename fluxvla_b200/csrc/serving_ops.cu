@@ -118,11 +118,13 @@ const void* cluster_kernel(int epi) {
     return reinterpret_cast<const void*>(G::gemm_fp8_cluster<FVB_EPI_GEGLU>);
   return reinterpret_cast<const void*>(G::gemm_fp8_cluster<FVB_EPI_F32_STORE>);
 }
+template <bool VEC>
 const void* pair_kernel(int epi) {
   namespace G = fvb::g8;
-  if (epi == FVB_EPI_BF16) return reinterpret_cast<const void*>(G::gemm_fp8_pair<FVB_EPI_BF16>);
-  if (epi == FVB_EPI_GEGLU) return reinterpret_cast<const void*>(G::gemm_fp8_pair<FVB_EPI_GEGLU>);
-  return reinterpret_cast<const void*>(G::gemm_fp8_pair<FVB_EPI_F32_STORE>);
+  if (epi == FVB_EPI_BF16) return reinterpret_cast<const void*>(G::gemm_fp8_pair<FVB_EPI_BF16, VEC>);
+  if (epi == FVB_EPI_GEGLU)
+    return reinterpret_cast<const void*>(G::gemm_fp8_pair<FVB_EPI_GEGLU, VEC>);
+  return reinterpret_cast<const void*>(G::gemm_fp8_pair<FVB_EPI_F32_STORE, VEC>);
 }
 
 // Clusters of 1..8 CTAs of the cluster kernel (one CTA per SM) that the device
@@ -304,7 +306,7 @@ int fvb_gemm_fp8(const fvb_gemm_fp8_args* a, void* stream) {
   d.sb = a->b_scale; d.ld_sb = a->ld_bs;
   d.out = a->out; d.ldo = a->ldo;
   const int eb = a->epilogue == FVB_EPI_F32_STORE ? 4 : 2;
-  d.vec_out = aligned16(a->out) && a->ldo * eb % 16 == 0;
+  d.vec_out = aligned16(a->out) && a->ldo * eb % 16 == 0 && nf * eb % 16 == 0 && a->n % 8 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   // The shape with the least time by a count of clocks, fitted to measured
   // products: a group costs the cluster kernel 600 clocks and a tile 4500
@@ -342,7 +344,8 @@ int fvb_gemm_fp8(const fvb_gemm_fp8_args* a, void* stream) {
     r = make_map_u8(&mt, a->a, a->m, a->k, a->lda, 128);
     if (r) return r;
     const int pairs = (int)(f_pair * t_pair < slots[2] ? f_pair * t_pair : slots[2]);
-    return launch_gemm_fp8(pair_kernel(a->epilogue), mt, mf, d, 2 * pairs, 2,
+    const void* two = d.vec_out ? pair_kernel<true>(a->epilogue) : pair_kernel<false>(a->epilogue);
+    return launch_gemm_fp8(two, mt, mf, d, 2 * pairs, 2,
                            fvb::g8::PairCfg::SMEM, st);
   }
   // tiles of equal height
