@@ -10,12 +10,13 @@
 // factor sa * sb of a group is one register for all its columns.  (With the
 // features there, few tokens would not waste rows of the tensor core, but the
 // factor would vary along the columns and come from shared memory for every
-// product: 13.7 us against 11.5 us on 64 x 2048 x 16384.)
+// product: 13.7 us against 12.5 us on 64 x 2048 x 16384.)
 //
 //   warp 0      TMA producer: ring of (tokens, weights) tiles of 128-byte rows
-//   warps 1, 3  tcgen05.mma issuers, every other group each: one alone takes
-//               about 600 clocks for a group's waits, four MMAs and commits,
-//               more than a 128 x 128 product
+//   warp 1      tcgen05.mma issuer; the cluster kernel has a second one, warp 3,
+//               for every other group: one takes longer over a group's waits,
+//               MMAs and commits than a 128 x 128 product does (13.5 us
+//               against 12.5 us on 64 x 2048 x 16384)
 //   warp 2      factors, four groups at a time, two batches ahead
 //   warps 4..11 read TMEM (warp w: lanes 32*(w%4)..+31, half of the columns),
 //               multiply by the factors, accumulate
@@ -40,7 +41,7 @@ namespace fvb {
 namespace g8 {
 
 constexpr int GROUP = 128;
-constexpr int BATCH = 4;  // groups of one batch of column factors
+constexpr int BATCH = 4;  // groups of one batch of factors
 constexpr int THREADS = 384;
 constexpr int FACTOR_WARP = 2, FIRST_SUM_WARP = 4;
 
@@ -477,22 +478,31 @@ __global__ void __launch_bounds__(THREADS, 1)
     // rows that are not 16-byte aligned, or end inside the tile: consecutive
     // lanes write consecutive values
     constexpr int W = EPI == FVB_EPI_GEGLU ? 2 : 1;  // features of a value
-#pragma unroll 4
-    for (int e = threadIdx.x; e < per * (C::TILE / W); e += THREADS) {
-      const int r = e / (C::TILE / W), f = e % (C::TILE / W) * W;
-      if (t0 + my0 + r >= p.m || f0 + f >= p.n) continue;
-      float v[W];
+    constexpr int N = C::TILE / W / 32;              // values of a lane in a row
+    const int most = min(per, p.m - t0 - my0);
+    for (int r = warp; r < most; r += THREADS / 32) {
+      float v[N][W];
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        v[j] = part[r * C::PITCH + f + j];
-        for (int i = 1; i < cl; ++i) v[j] += part[(i * per + r) * C::PITCH + f + j];
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[i][j] = part[r * C::PITCH + (i * 32 + lane) * W + j];
+      for (int c = 1; c < cl; ++c)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int j = 0; j < W; ++j)
+            v[i][j] += part[(c * per + r) * C::PITCH + (i * 32 + lane) * W + j];
+      const long long at = (long long)(t0 + my0 + r) * p.ldo + f0 / W;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int f = i * 32 + lane;
+        if (f0 + f * W >= p.n) continue;
+        if (EPI == FVB_EPI_F32_STORE)
+          static_cast<float*>(p.out)[at + f] = v[i][0];
+        else
+          static_cast<bf16*>(p.out)[at + f] =
+              __float2bfloat16(EPI == FVB_EPI_GEGLU ? geglu(v[i][0], v[i][W - 1]) : v[i][0]);
       }
-      const long long at = (long long)(t0 + my0 + r) * p.ldo + (f0 + f) / W;
-      if (EPI == FVB_EPI_F32_STORE)
-        static_cast<float*>(p.out)[at] = v[0];
-      else
-        static_cast<bf16*>(p.out)[at] =
-            __float2bfloat16(EPI == FVB_EPI_GEGLU ? geglu(v[0], v[W - 1]) : v[0]);
     }
   }
   if (cl > 1) {
@@ -617,15 +627,15 @@ __global__ void __launch_bounds__(THREADS, 1)
           tma_load_2d_pair(sa + C::HALF, &tmB, g * GROUP, wrow, fb);
         }
       }
-    } else if ((warp == 1 || warp == 3) && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
       constexpr uint32_t IDESC = idesc_e4m3_f32(256, C::TILE);
       const bool elected = elect_one();
       const int n_it = p.groups * ((n_tiles - pair + n_pairs - 1) / n_pairs);
-      const int b = warp >> 1;  // accumulator of this issuer's groups
-      int s = b;
+      int s = 0;
       uint32_t phase = 0;
 #pragma unroll 1
-      for (int it = b; it < n_it; it += 2) {
+      for (int it = 0; it < n_it; ++it) {
+        const int b = it & 1;
         bool ready = mbar_wait_spin(&full[s], phase);
         ready = ready && mbar_wait_cluster(&tempty[b], ((it >> 1) & 1) ^ 1);
         if (!__all_sync(0xffffffffu, ready)) break;
@@ -640,9 +650,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           commit_both(&empty[s]);
         }
         __syncwarp();
-        s += 2;
-        if (s >= C::STAGES) {
-          s -= C::STAGES;
+        if (++s == C::STAGES) {
+          s = 0;
           phase ^= 1;
         }
       }
