@@ -22,9 +22,10 @@
 //               multiply by the factors, accumulate
 //
 // Two kernels:
-//   gemm_fp8_cluster  up to 128 tokens x 128 features a CTA, the groups split
-//                     over the CTAs of a cluster: enough CTAs to fill the GPU
-//                     however few the tiles are.  The partial tiles are
+//   gemm_fp8_cluster  tiles of up to 128 tokens x 128 features, several to a CTA
+//                     one after the other, or one to a cluster, whose CTAs
+//                     split the groups: enough CTAs to fill the GPU however
+//                     few the tiles are.  The partial tiles are
 //                     exchanged through distributed shared memory and summed
 //                     in the order of the groups, so a product is the same
 //                     from call to call and needs no workspace.
@@ -249,7 +250,7 @@ __device__ __forceinline__ float pick(const float4& v, int e) {
 }
 
 // ---------------------------------------------------------------------------
-// one tile per CTA, groups split over a cluster
+// tiles of one SM, or of a cluster that splits the groups
 // ---------------------------------------------------------------------------
 struct ClusterCfg {
   static constexpr int TILE = 128;                  // features (and most tokens)
@@ -274,7 +275,66 @@ struct ClusterCfg {
   static int smem(int rows) { return fixed_bytes(rows) + stages(rows) * stage_bytes(rows); }
 };
 
+// Sums `cl` partials [per rows][PITCH] and writes them as token rows t0.. and
+// features f0..; threads tid of n.
 template <int EPI>
+__device__ __forceinline__ void write_tile(const Dev& p, const float* part, int cl, int per, int t0,
+                                           int f0, int tid, int n) {
+  using C = ClusterCfg;
+  const int lane = tid & 31;
+  auto sum4 = [&](int r, int f) {
+    float4 v = *reinterpret_cast<const float4*>(part + r * C::PITCH + f);
+    for (int i = 1; i < cl; ++i) {
+      const float4 w = *reinterpret_cast<const float4*>(part + (i * per + r) * C::PITCH + f);
+      v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+    }
+    return v;
+  };
+  if (p.vec_out) {
+#pragma unroll 2
+    for (int e = tid; e < per * (C::TILE / 8); e += n) {
+      const int r = e / (C::TILE / 8), f = e % (C::TILE / 8) * 8;
+      const float4 a = sum4(r, f), b = sum4(r, f + 4);
+      const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      if (t0 + r < p.m && f0 + f < p.n) store8<EPI>(p, t0 + r, f0 + f, v);
+    }
+  } else {
+    // rows that are not 16-byte aligned, or end inside the tile: consecutive
+    // lanes write consecutive values
+    constexpr int W = EPI == FVB_EPI_GEGLU ? 2 : 1;  // features of a value
+    constexpr int N = C::TILE / W / 32;              // values of a lane in a row
+    const int most = min(per, p.m - t0);
+    for (int r = tid >> 5; r < most; r += n >> 5) {
+      float v[N][W];
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[i][j] = part[r * C::PITCH + (i * 32 + lane) * W + j];
+      for (int c = 1; c < cl; ++c)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int j = 0; j < W; ++j)
+            v[i][j] += part[(c * per + r) * C::PITCH + (i * 32 + lane) * W + j];
+      const long long at = (long long)(t0 + r) * p.ldo + f0 / W;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int f = i * 32 + lane;
+        if (f0 + f * W >= p.n) continue;
+        if (EPI == FVB_EPI_F32_STORE)
+          static_cast<float*>(p.out)[at + f] = v[i][0];
+        else
+          static_cast<bf16*>(p.out)[at + f] =
+              __float2bfloat16(EPI == FVB_EPI_GEGLU ? geglu(v[i][0], v[i][W - 1]) : v[i][0]);
+      }
+    }
+  }
+}
+
+// MULTI: a CTA has every gridDim.x-th tile (cl = 1); else one tile, its own or
+// its cluster's.  (One kernel for both starts 0.7 us later on the small
+// products.)
+template <int EPI, bool MULTI>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_fp8_cluster(const __grid_constant__ CUtensorMap tmA,
                      const __grid_constant__ CUtensorMap tmB, const Dev p) {
@@ -299,8 +359,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cl = p.cl;
   const int rank = cl > 1 ? (int)cluster_rank() : 0;
-  const int tile = blockIdx.x / cl;
-  const int f0 = tile % p.f_tiles * C::TILE, t0 = tile / p.f_tiles * rows;
+  const int tile0 = blockIdx.x / cl, n_tiles = p.f_tiles * p.t_tiles;
+  const int stride = gridDim.x;  // MULTI
+  const int my_tiles = MULTI ? (n_tiles - tile0 + stride - 1) / stride : 1;
+  const int f0 = tile0 % p.f_tiles * C::TILE, t0 = tile0 / p.f_tiles * rows;  // of the first
   const int g0 = (int)((long long)p.groups * rank / cl);
   const int g1 = (int)((long long)p.groups * (rank + 1) / cl);
   const int ng = g1 - g0;
@@ -339,17 +401,22 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (lane == 0) {
       int s = 0;
       uint32_t phase = 1;
-      for (int i = 0; i < ng; ++i) {
-        if (!mbar_wait_spin(&empty[s], phase)) break;
-        mbar_arrive_expect_tx(&full[s], stage_bytes);
-        uint8_t* st = smem + s * stage_bytes;
-        tma_load_2d(st + a_bytes, &tmB, (g0 + i) * GROUP, f0, &full[s]);
-        tma_load_2d(st, &tmA, (g0 + i) * GROUP, t0, &full[s]);
-        if (++s == stages) {
-          s = 0;
-          phase ^= 1;
+      bool alive = true;
+      int w = tile0;
+      do {
+        const int f = w % p.f_tiles * C::TILE, t = w / p.f_tiles * rows;
+        for (int g = g0; g < g1; ++g) {
+          if (!mbar_wait_spin(&empty[s], phase)) { alive = false; break; }
+          mbar_arrive_expect_tx(&full[s], stage_bytes);
+          uint8_t* st = smem + s * stage_bytes;
+          tma_load_2d(st + a_bytes, &tmB, g * GROUP, f, &full[s]);
+          tma_load_2d(st, &tmA, g * GROUP, t, &full[s]);
+          if (++s == stages) {
+            s = 0;
+            phase ^= 1;
+          }
         }
-      }
+      } while (MULTI && alive && (w += stride) < n_tiles);
     }
     __syncwarp();
     if (cl > 1) cluster_wait();
@@ -361,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     int s = first % stages;
     uint32_t phase = (first / stages) & 1;
 #pragma unroll 1
-    for (int i = first; i < ng; i += 2) {
+    for (int i = first; i < ng * my_tiles; i += 2) {
       const int b = i % NB;
       bool ready = mbar_wait_spin(&full[s], phase);
       ready = ready && mbar_wait_spin(&tempty[b], ((i / NB) & 1) ^ 1);
@@ -386,58 +453,96 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (cl > 1) cluster_wait();
   } else if (warp == FACTOR_WARP) {
     int bt = 0;
-    write_factors<1>(p, t0, f0 / 128, g0, g1, fac, ffull, fempty, bt, lane);
+    int w = tile0;
+    bool alive;
+    do {
+      alive = write_factors<1>(p, w / p.f_tiles * rows, w % p.f_tiles, g0, g1, fac, ffull, fempty,
+                               bt, lane);
+    } while (MULTI && alive && (w += stride) < n_tiles);
     if (cl > 1) cluster_wait();
   } else {
     const int q = warp & 3, half = (warp - FIRST_SUM_WARP) >> 2;
     const bool used = q * 32 < rows;  // lanes past the last row are not read
-    float acc[COLS];
-#pragma unroll
-    for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
     const uint32_t lane_base = tmem + ((uint32_t)(q * 32) << 16) + half * COLS;
+    // the eight summing warps meet; true if none has given up a wait
+    auto sum_barrier = [](bool fine) {
+      uint32_t all;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\t"
+          "setp.ne.u32 p, %1, 0;\n\t"
+          "bar.red.and.pred q, 1, 256, p;\n\t"
+          "selp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(all)
+          : "r"((uint32_t)fine)
+          : "memory");
+      return all != 0;
+    };
+    float acc[COLS];
     bool ok = true;
-    for (int i0 = 0; i0 < ng && ok; i0 += BATCH) {
-      const int slot = (i0 / BATCH) & 1;
-      ok = mbar_wait_spin(&ffull[slot], (i0 / (2 * BATCH)) & 1);
-      const float4 f4 = reinterpret_cast<const float4*>(fac)[slot * 128 + q * 32 + lane];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&fempty[slot]);
+    int it = 0, bt = 0, w = tile0;
+    do {
 #pragma unroll
-      for (int e = 0; e < BATCH; ++e) {
-        const int i = i0 + e, b = i % NB;
-        if (i < ng && ok) {
-          ok = mbar_wait_spin(&tfull[b], (i / NB) & 1);
-          ok = __all_sync(0xffffffffu, ok);
-          if (ok) {
-            tc_fence_after();
-            uint32_t r[COLS];
-            if (used) {
+      for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
+      for (int i0 = 0; i0 < ng && ok; i0 += BATCH) {
+        const int batch = MULTI ? bt++ : i0 / BATCH, slot = batch & 1;
+        ok = mbar_wait_spin(&ffull[slot], (batch >> 1) & 1);
+        const float4 f4 = reinterpret_cast<const float4*>(fac)[slot * 128 + q * 32 + lane];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&fempty[slot]);
 #pragma unroll
-              for (int j = 0; j < COLS; j += 32) tmem_ld32(lane_base + b * C::TILE + j, r + j);
-              tmem_wait<COLS>(r);
+        for (int e = 0; e < BATCH; ++e) {
+          if (i0 + e < ng && ok) {
+            static_assert(NB == BATCH, "a batch starts at the first accumulator");
+            const int b = MULTI ? it % NB : e;
+            ok = mbar_wait_spin(&tfull[b], (MULTI ? it / NB : i0 / NB) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+              tc_fence_after();
+              uint32_t r[COLS];
+              if (used) {
+#pragma unroll
+                for (int j = 0; j < COLS; j += 32) tmem_ld32(lane_base + b * C::TILE + j, r + j);
+                tmem_wait<COLS>(r);
+              }
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&tempty[b]);
+              if (used) scale_add<COLS>(acc, r, pick(f4, e));
+              if (MULTI) ++it;
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&tempty[b]);
-            if (used) scale_add<COLS>(acc, r, pick(f4, e));
           }
         }
       }
-    }
-    // every product has been read, so the ring is free: the partial tile goes
-    // there, and each CTA's token rows in one copy to that CTA
-    if (q * 32 + lane < rows) {
-      float* t = reinterpret_cast<float*>(smem) + (q * 32 + lane) * C::PITCH + half * COLS;
+      if (!MULTI) break;  // written below
+      // the tile goes through the space for received partials, while the next
+      // tile's products are under way
+      if (ok && q * 32 + lane < rows) {
+        float* t = reinterpret_cast<float*>(recv) + (q * 32 + lane) * C::PITCH + half * COLS;
 #pragma unroll
-      for (int j = 0; j < COLS; j += 4)
-        *reinterpret_cast<float4*>(t + j) =
-            make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-    }
-    fence_proxy_async_smem();
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (cl > 1) {
-      cluster_wait();
-      if (warp == FIRST_SUM_WARP && lane < cl && ok) {
+        for (int j = 0; j < COLS; j += 4)
+          *reinterpret_cast<float4*>(t + j) =
+              make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+      }
+      ok = sum_barrier(ok);
+      if (ok)
+        write_tile<EPI>(p, reinterpret_cast<const float*>(recv), 1, rows, w / p.f_tiles * rows,
+                        w % p.f_tiles * C::TILE, threadIdx.x - 32 * FIRST_SUM_WARP, 256);
+      sum_barrier(ok);
+    } while (ok && (w += stride) < n_tiles);
+    if (!MULTI) {
+      // every product has been read, so the ring is free: the partial tile goes
+      // there, and each CTA's token rows in one copy to that CTA
+      if (q * 32 + lane < rows) {
+        float* t = reinterpret_cast<float*>(smem) + (q * 32 + lane) * C::PITCH + half * COLS;
+#pragma unroll
+        for (int j = 0; j < COLS; j += 4)
+          *reinterpret_cast<float4*>(t + j) =
+              make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+      }
+      fence_proxy_async_smem();
+      ok = sum_barrier(ok);
+      if (cl > 1) cluster_wait();
+      if (warp == FIRST_SUM_WARP && lane < cl && cl > 1 && ok) {
         const int to = rows * lane / cl;  // first row of the CTA that this lane serves
         const uint32_t bytes = C::part_bytes(rows * (lane + 1) / cl - to);
         asm volatile(
@@ -455,56 +560,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_after();
     tmem_dealloc(tmem, NB * C::TILE);
   }
+  if (MULTI) return;
   // this CTA's tokens: the cluster's partials in the order of the groups
-  const float* part = reinterpret_cast<const float*>(cl > 1 ? recv : smem);
   if (cl > 1) mbar_wait_cluster(recvd, 0);
-  auto sum4 = [&](int r, int f) {
-    float4 v = *reinterpret_cast<const float4*>(part + r * C::PITCH + f);
-    for (int i = 1; i < cl; ++i) {
-      const float4 w = *reinterpret_cast<const float4*>(part + (i * per + r) * C::PITCH + f);
-      v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
-    }
-    return v;
-  };
-  if (p.vec_out) {
-#pragma unroll 2
-    for (int e = threadIdx.x; e < per * (C::TILE / 8); e += THREADS) {
-      const int r = e / (C::TILE / 8), f = e % (C::TILE / 8) * 8;
-      const float4 a = sum4(r, f), b = sum4(r, f + 4);
-      const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-      if (t0 + my0 + r < p.m && f0 + f < p.n) store8<EPI>(p, t0 + my0 + r, f0 + f, v);
-    }
-  } else {
-    // rows that are not 16-byte aligned, or end inside the tile: consecutive
-    // lanes write consecutive values
-    constexpr int W = EPI == FVB_EPI_GEGLU ? 2 : 1;  // features of a value
-    constexpr int N = C::TILE / W / 32;              // values of a lane in a row
-    const int most = min(per, p.m - t0 - my0);
-    for (int r = warp; r < most; r += THREADS / 32) {
-      float v[N][W];
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int j = 0; j < W; ++j) v[i][j] = part[r * C::PITCH + (i * 32 + lane) * W + j];
-      for (int c = 1; c < cl; ++c)
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-          for (int j = 0; j < W; ++j)
-            v[i][j] += part[(c * per + r) * C::PITCH + (i * 32 + lane) * W + j];
-      const long long at = (long long)(t0 + my0 + r) * p.ldo + f0 / W;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int f = i * 32 + lane;
-        if (f0 + f * W >= p.n) continue;
-        if (EPI == FVB_EPI_F32_STORE)
-          static_cast<float*>(p.out)[at + f] = v[i][0];
-        else
-          static_cast<bf16*>(p.out)[at + f] =
-              __float2bfloat16(EPI == FVB_EPI_GEGLU ? geglu(v[i][0], v[i][W - 1]) : v[i][0]);
-      }
-    }
-  }
+  write_tile<EPI>(p, reinterpret_cast<const float*>(cl > 1 ? recv : smem), cl, per, t0 + my0, f0,
+                  threadIdx.x, THREADS);
   if (cl > 1) {
     // the copies out of this CTA have been received everywhere
     cluster_arrive();

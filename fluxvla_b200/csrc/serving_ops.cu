@@ -111,12 +111,14 @@ int launch_gemm_fp8(const void* kern, const CUtensorMap& ma, const CUtensorMap& 
   return check_launch("fvb_gemm_fp8");
 }
 
+template <bool MULTI>
 const void* cluster_kernel(int epi) {
   namespace G = fvb::g8;
-  if (epi == FVB_EPI_BF16) return reinterpret_cast<const void*>(G::gemm_fp8_cluster<FVB_EPI_BF16>);
+  if (epi == FVB_EPI_BF16)
+    return reinterpret_cast<const void*>(G::gemm_fp8_cluster<FVB_EPI_BF16, MULTI>);
   if (epi == FVB_EPI_GEGLU)
-    return reinterpret_cast<const void*>(G::gemm_fp8_cluster<FVB_EPI_GEGLU>);
-  return reinterpret_cast<const void*>(G::gemm_fp8_cluster<FVB_EPI_F32_STORE>);
+    return reinterpret_cast<const void*>(G::gemm_fp8_cluster<FVB_EPI_GEGLU, MULTI>);
+  return reinterpret_cast<const void*>(G::gemm_fp8_cluster<FVB_EPI_F32_STORE, MULTI>);
 }
 template <bool VEC>
 const void* pair_kernel(int epi) {
@@ -137,7 +139,7 @@ const int* cluster_slots() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) dev = 0;
   std::lock_guard<std::mutex> lk(mu);
   if (slots[dev][1]) return slots[dev];
-  const void* kern = cluster_kernel(FVB_EPI_BF16);
+  const void* kern = cluster_kernel<false>(FVB_EPI_BF16);
   for (int c = 8; c >= 1; --c) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(c * 256);
@@ -309,13 +311,11 @@ int fvb_gemm_fp8(const fvb_gemm_fp8_args* a, void* stream) {
   d.vec_out = aligned16(a->out) && a->ldo * eb % 16 == 0 && nf * eb % 16 == 0 && a->n % 8 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   // The shape with the least time by a count of clocks, fitted to measured
-  // products: a group costs the cluster kernel 600 clocks and a tile 4500
-  // (6000 with an exchange), the pair kernel 970 and 3500 for a tile of twice
-  // the height and width.  816 x 32768 x 2048: pair 70 us, clusters 109 us;
+  // products: a group costs the cluster kernel 600 clocks, a call 3000, a tile
+  // 1500 more (3000 with an exchange), the pair kernel 970 and 3500 for a tile
+  // of twice the height and width.  816 x 32768 x 2048: pair 70 us, clusters 109 us;
   // 816 x 2560 x 2048: the other way round, 40 pair tiles leave SMs idle.
-  const void* kern = cluster_kernel(a->epilogue);
-  if (int rr = ensure_smem(kern, fvb::g8::ClusterCfg::MAX_SMEM, "fvb_gemm_fp8")) return rr;
-  if (int rr = ensure_smem(cluster_kernel(FVB_EPI_BF16), fvb::g8::ClusterCfg::MAX_SMEM,
+  if (int rr = ensure_smem(cluster_kernel<false>(FVB_EPI_BF16), fvb::g8::ClusterCfg::MAX_SMEM,
                            "fvb_gemm_fp8"))
     return rr;
   const int* slots = cluster_slots();
@@ -327,7 +327,8 @@ int fvb_gemm_fp8(const fvb_gemm_fp8_args* a, void* stream) {
   d.cl = 1;
   for (int c = 1; c <= 8 && c <= groups; ++c) {
     if (!slots[c]) continue;
-    const int64_t t = waves(tiles, slots[c]) * ((groups + c - 1) / c * 600 + (c > 1 ? 6000 : 4500));
+    const int64_t t = c > 1 ? waves(tiles, slots[c]) * ((groups + c - 1) / c * 600 + 6000)
+                            : waves(tiles, slots[1]) * (groups * 600 + 1500) + 3000;
     if (t < best) {
       best = t;
       d.cl = c;
@@ -354,7 +355,10 @@ int fvb_gemm_fp8(const fvb_gemm_fp8_args* a, void* stream) {
   d.stages = fvb::g8::ClusterCfg::stages(d.rows);
   r = make_map_u8(&mt, a->a, a->m, a->k, a->lda, d.rows);
   if (r) return r;
-  return launch_gemm_fp8(kern, mt, mf, d, (int)tiles * d.cl, d.cl,
+  const int ctas = d.cl > 1 ? (int)tiles * d.cl : (int)(tiles < slots[1] ? tiles : slots[1]);
+  const bool multi = d.cl == 1 && tiles > ctas;
+  const void* kern = multi ? cluster_kernel<true>(a->epilogue) : cluster_kernel<false>(a->epilogue);
+  return launch_gemm_fp8(kern, mt, mf, d, ctas, d.cl,
                          fvb::g8::ClusterCfg::smem(d.rows), st);
 }
 

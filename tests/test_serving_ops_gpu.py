@@ -213,7 +213,8 @@ EPIS = {'bf16': _lib.EPI_BF16, 'f32': _lib.EPI_F32_STORE,
     (17, 1152, 4304), (33, 254, 1000), (51, 1024, 4096), (64, 2048, 16384),
     (65, 128, 256), (100, 514, 640), (128, 256, 128), (129, 130, 272),
     (300, 1152, 1152), (816, 2560, 2048), (257, 4098, 1040),
-    (1500, 4100, 272), (2049, 8194, 1000), (8, 384, 5000), (4000, 2, 16)])
+    (1500, 4100, 272), (2049, 8194, 1000), (8, 384, 5000), (4000, 2, 16),
+    (7, 20002, 528), (70, 38000, 130)])
 def test_gemm_fp8(epi, m, n, k):
     g = gen(m + 3 * n + 7 * k)
     kp = -(-k // 16) * 16          # rows of 16-byte multiples
