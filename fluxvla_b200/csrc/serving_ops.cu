@@ -245,6 +245,9 @@ int fvb_norm_fp8(const fvb_norm_fp8_args* a, void* stream) {
   if (a->mode != FVB_NORM_NONE && a->dim > FVB_NORM_FP8_MAX_DIM)
     return fail(FVB_ERR_UNSUPPORTED, "fvb_norm_fp8: dim %d over %d", a->dim,
                 FVB_NORM_FP8_MAX_DIM);
+  // without one, 2^11 columns to a CTA and 2^16 - 1 CTAs to a row
+  if (a->dim > 65535 * 2048)
+    return fail(FVB_ERR_UNSUPPORTED, "fvb_norm_fp8: dim %d over %d", a->dim, 65535 * 2048);
   if (!a->x || !a->q || !a->scales)
     return fail(FVB_ERR_INVALID_ARG, "fvb_norm_fp8: NULL operand");
   if (a->mode == FVB_NORM_GEMMA_RMS && !a->w)
@@ -291,6 +294,10 @@ int fvb_gemm_fp8(const fvb_gemm_fp8_args* a, void* stream) {
     return fail(FVB_ERR_INVALID_ARG, "fvb_gemm_fp8: bad epilogue %d", a->epilogue);
   if (a->epilogue == FVB_EPI_GEGLU && a->n % 2)
     return fail(FVB_ERR_INVALID_ARG, "fvb_gemm_fp8: GEGLU needs an even feature count");
+  // rows of the last tile are counted past the last token and feature
+  constexpr int MOST = INT32_MAX - 256;
+  if (a->m > MOST || a->n > MOST || a->k > MOST)
+    return fail(FVB_ERR_UNSUPPORTED, "fvb_gemm_fp8: too large");
   if (!a->a || !a->a_scale || !a->b || !a->b_scale || !a->out)
     return fail(FVB_ERR_INVALID_ARG, "fvb_gemm_fp8: NULL operand");
   const int groups = (a->k + 127) / 128;

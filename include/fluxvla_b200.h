@@ -313,7 +313,7 @@ int fvb_norm_bf16(int32_t mode, const void* x, int64_t ld_in, void* out,
  * contiguous cache with bf16 weights.
  * ------------------------------------------------------------------------- */
 
-/* Largest row of fvb_norm_fp8 with a norm (FVB_NORM_NONE has no limit). */
+/* Largest row of fvb_norm_fp8 with a norm (FVB_NORM_NONE: 65535 * 2048). */
 #define FVB_NORM_FP8_MAX_DIM 16384
 
 typedef struct fvb_norm_fp8_args {

@@ -35,6 +35,8 @@ def norm_args():
     (dict(rows=-1), 'bad shape', 1), (dict(dim=0), 'bad shape', 1),
     (dict(mode=_lib.NORM_LAYER), 'bad mode', 1), (dict(mode=6), 'bad mode', 1),
     (dict(dim=16385, ld_x=16385, ld_q=16385, ld_scales=129), 'over 16384', 2),
+    (dict(mode=_lib.NORM_NONE, dim=2 ** 31 - 1, ld_x=2 ** 31, ld_q=2 ** 31,
+          ld_scales=2 ** 24), 'over 134215680', 2),
     (dict(x=None), 'NULL', 1), (dict(q=None), 'NULL', 1),
     (dict(scales=None), 'NULL', 1),
     (dict(mode=_lib.NORM_GEMMA_RMS), 'weight required', 1),
@@ -68,6 +70,15 @@ def gemm_args():
     (dict(b=P + 1), '16B aligned')])
 def test_gemm_fp8_refusals(kw, text):
     refused('fvb_gemm_fp8', with_(gemm_args(), **kw), text)
+
+
+@pytest.mark.parametrize('kw', [
+    dict(m=2 ** 31 - 1), dict(n=2 ** 31 - 1, ldo=2 ** 31),
+    dict(k=2 ** 31 - 1, lda=2 ** 31, ldb=2 ** 31, ld_as=2 ** 24,
+         ld_bs=2 ** 24)])
+def test_gemm_fp8_sizes_at_the_end_of_32_bits(kw):
+    refused('fvb_gemm_fp8', with_(gemm_args(), **kw), 'too large',
+            _lib.FVB_ERR_UNSUPPORTED)
 
 
 def append_args():
