@@ -12,7 +12,9 @@
 // against 6.5 us of memory traffic), so 64 bits are used where they decide:
 // the row's sum of squares, the group's largest value, and those vectors of
 // which a value, computed to 32 bits with its error bound, has a border inside
-// the bound (about one in ten thousand).
+// the bound (about one in ten thousand).  Without a norm y is what 32 bits
+// hold, and y / s rounded to odd takes their place: 10.5 us on 848 x 16384,
+// bound by the issue of instructions.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -130,28 +132,40 @@ __device__ __forceinline__ float off_border(float t, double y, double s) {
   return t;
 }
 
-// The same for a value y that f32 holds: t = |y| / s within 2^-21.  A border
-// that near is decided by y - border * s, whose sign one rounding keeps.  bf16
-// values meet borders exactly in every group whose largest value is a multiple
-// of 7, so this path has no 64-bit arithmetic.
-__device__ __forceinline__ float off_border(float t, float y, float s) {
-  const uint32_t b = __float_as_uint(t);
-  float border;
-  bool close;
-  if (b >= 0x3c7ffff0u) {  // 2^-6, less the bound
-    border = __uint_as_float((b & 0xfff00000u) | 0x80000u);
-    close = (b & 0xfffffu) - 0x7fff0u <= 0x20u;
-  } else {
-    const float r = t * 1024.f, odd = 2.f * floorf(0.5f * r) + 1.f;
-    border = odd * 0x1p-10f;
-    close = fabsf(r - odd) <= r * 0x1p-20f;
-  }
-  if (close) {
-    const float d = fmaf(-border, s, y);
-    const uint32_t c = __float_as_uint(border);
-    t = __uint_as_float(d > 0.f ? c + 1 : (d < 0.f ? c - 1 : c));
-  }
-  return t;
+// Two 32-bit values to an instruction.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(f32x2 v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// y / s rounded to odd (toward zero, and the last bit set where that was not
+// exact), which rounds to e4m3 as y / s itself does; y0, y1 >= 0 that f32
+// holds, r = 1 / s within an ulp.  t is the quotient within its last bit, so
+// that the remainder y - t s, rounded once, has the sign of the error.
+__device__ __forceinline__ void divide_odd(float y0, float y1, float s, float r, float& t0,
+                                           float& t1) {
+  const f32x2 y = pair(y0, y1), ns = pair(-s, -s), r2 = pair(r, r);
+  const f32x2 q = mul2(y, r2), t = fma2(fma2(ns, q, y), r2, q);
+  float d0, d1;
+  unpair(fma2(ns, t, y), d0, d1);
+  unpair(t, t0, t1);
+  t0 = __uint_as_float((__float_as_uint(t0) - (d0 < 0.f)) | (d0 != 0.f));
+  t1 = __uint_as_float((__float_as_uint(t1) - (d1 < 0.f)) | (d1 != 0.f));
 }
 
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
@@ -166,22 +180,37 @@ __device__ __forceinline__ float rcp(float x) {  // within an ulp
   return y;
 }
 
-// largest of the 16 lanes that share a scale; values not negative
+// largest of the N lanes that share a scale; values not negative
+template <int N = LANES>
 __device__ __forceinline__ float group_max(float v) {
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = N / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
+// the first n of 8 codes to columns c.. of a row
+__device__ __forceinline__ void store_codes(const Dev& p, long long row, int c, int n, uint32_t lo,
+                                            uint32_t hi) {
+  uint8_t* q = p.q + row * p.ld_q + c;
+  if (p.vec && n == 8) {
+    *reinterpret_cast<uint2*>(q) = make_uint2(lo, hi);
+  } else {
+    for (int j = 0; j < n; ++j) q[j] = static_cast<uint8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
+  }
+}
+
 // One row (or, without a norm, one run of columns of a row) per CTA; thread t
-// holds VPT vectors of 8 columns, so 16 neighbouring lanes share a scale.
+// holds VPT vectors of 8 columns.  With a norm these are T vectors apart and 16
+// neighbouring lanes share a scale; without one they are neighbours, and 16 /
+// VPT lanes do.
 template <typename TX, int DT, int VPT, int KIND>
 __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_kernel(const Dev p) {
   constexpr bool NORM = KIND != CODES, ADA = KIND == SHIFT;
   __shared__ double part[MAX_THREADS / 32];
   const int T = blockDim.x, tid = threadIdx.x, lane = tid & 31;
   const long long row = blockIdx.x;
-  const int c0 = (blockIdx.y * VPT * T + tid) * VEC;
+  const int c0 = (blockIdx.y * T + tid) * VEC * (NORM ? 1 : VPT);
+  const int step = NORM ? T * VEC : VEC;  // from a thread's vector to its next
   const bool vec = p.vec;
   const TX* x = static_cast<const TX*>(p.x) + row * p.ld_x;
   griddep_wait();
@@ -189,13 +218,13 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
   float h[VPT][8];
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    const int c = c0 + v * T * VEC;
+    const int c = c0 + v * step;
     load8(x + c, min(max(p.dim - c, 0), VEC), vec, h[v]);
   }
   if (DT != DELTA_NONE) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int c = c0 + v * T * VEC;
+      const int c = c0 + v * step;
       const int n = min(max(p.dim - c, 0), VEC);
       float d[8];
       if (DT == DELTA_F32)
@@ -207,8 +236,42 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
       store8(static_cast<TX*>(p.res) + row * p.ld_res + c, n, vec, h[v]);
     }
   }
+  if (!NORM) {
+    float top = static_cast<float>(MIN_AMAX);  // fmax drops NaN: the others keep their codes
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(h[v][j]));
+    // top / 448 rounded to f32, by a multiplication and its remainder
+    // (Markstein); infinity stays infinity
+    top = group_max<LANES / VPT>(top);
+    constexpr float M = static_cast<float>(E4M3_MAX), I = 1.f / M;
+    const float q = top * I;
+    const float s = top < INFINITY ? fmaf(fmaf(-M, q, top), I, q) : top;
+    const float r = rcp(s);
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int c = c0 + v * step;
+      float t[8];
+      if (s < INFINITY) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2)
+          divide_odd(fabsf(h[v][j]), fabsf(h[v][j + 1]), s, r, t[j], t[j + 1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = fabsf(h[v][j]) * 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] = copysignf(t[j], h[v][j]);
+      store_codes(p, row, c, min(p.dim - c, VEC), codes4(t[0], t[1], t[2], t[3]),
+                  codes4(t[4], t[5], t[6], t[7]));
+    }
+    if ((lane & (LANES / VPT - 1)) == 0 && c0 < p.dim)
+      p.scales[row * p.ld_scales + c0 / GROUP] = s;
+    return;
+  }
   double rstd = 1.0;
-  if (NORM) {
+  {
     double ss = 0.0;
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
@@ -228,10 +291,10 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
   const float rf = static_cast<float>(rstd);
   // near the ends of the 32-bit range the bounds do not hold (nor where rf is
   // NaN): such rows are computed in 64 bits throughout
-  const bool fine = !NORM || (rf >= 0x1p-100f && rf <= 0x1p100f);
+  const bool fine = rf >= 0x1p-100f && rf <= 0x1p100f;
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    const int c = c0 + v * T * VEC;
+    const int c = c0 + v * step;
     const int n = min(max(p.dim - c, 0), VEC);
     // y to 32 bits, and what bounds its error: EPS * mag
     float y[8], mag[8], w[8], b[8];
@@ -248,7 +311,7 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      y[j] = NORM ? h[v][j] * rf * (1.f + w[j]) : h[v][j];
+      y[j] = h[v][j] * rf * (1.f + w[j]);
       mag[j] = fabsf(y[j]);
       if (ADA) {
         mag[j] += fabsf(b[j]);
@@ -256,45 +319,31 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
       }
     }
     auto exact = [&](int j) {
-      double r = h[v][j];
-      if (NORM) r = r * rstd * (1.0 + w[j]);
+      double r = h[v][j] * rstd * (1.0 + w[j]);
       if (ADA) r += b[j];
       return r;
     };
-    float s;
-    if (NORM) {
-      // of the values that may be the largest, the largest scale
-      float low = 0.f, high = 0.f;  // fmax drops NaN: the others keep their codes
+    // of the values that may be the largest, the largest scale
+    float low = 0.f, high = 0.f;  // fmax drops NaN: the others keep their codes
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float a = fabsf(y[j]);
-        low = fmaxf(low, ADA ? fmaf(-EPS, mag[j], a) : a);
-        high = fmaxf(high, ADA ? fmaf(EPS, mag[j], a) : a);
-      }
-      if (!ADA) {
-        low *= 1.f - EPS;
-        high *= 1.f + EPS;
-      }
-      low = group_max(low);
-      s = static_cast<float>(MIN_AMAX / E4M3_MAX);
-      if (!fine || (high >= low && low > 0.f)) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (!fine || fmaf(EPS, mag[j], fabsf(y[j])) >= low)
-            s = fmaxf(s, static_cast<float>(fabs(exact(j)) * (1.0 / E4M3_MAX)));
-      }
-      s = group_max(s);
-    } else {
-      float top = static_cast<float>(MIN_AMAX);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmaxf(top, mag[j]);
-      // top / 448 rounded to f32, by a multiplication and its remainder
-      // (Markstein); infinity stays infinity
-      top = group_max(top);
-      constexpr float M = static_cast<float>(E4M3_MAX), I = 1.f / M;
-      const float q = top * I;
-      s = top < INFINITY ? fmaf(fmaf(-M, q, top), I, q) : top;
+    for (int j = 0; j < 8; ++j) {
+      const float a = fabsf(y[j]);
+      low = fmaxf(low, ADA ? fmaf(-EPS, mag[j], a) : a);
+      high = fmaxf(high, ADA ? fmaf(EPS, mag[j], a) : a);
     }
+    if (!ADA) {
+      low *= 1.f - EPS;
+      high *= 1.f + EPS;
+    }
+    low = group_max(low);
+    float s = static_cast<float>(MIN_AMAX / E4M3_MAX);
+    if (!fine || (high >= low && low > 0.f)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (!fine || fmaf(EPS, mag[j], fabsf(y[j])) >= low)
+          s = fmaxf(s, static_cast<float>(fabs(exact(j)) * (1.0 / E4M3_MAX)));
+    }
+    s = group_max(s);
     if (n <= 0) continue;
     // codes of both ends of each value's interval
     const float r = rcp(s), r_lo = r * (1.f - EPS), r_hi = r * (1.f + EPS);
@@ -308,26 +357,16 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
     if (!fine || code[0] != codes4(hi[0], hi[1], hi[2], hi[3]) ||
         code[1] != codes4(hi[4], hi[5], hi[6], hi[7])) {
       float t[8];
-      if (NORM) {
-        const double sd = s, inv = 1.0 / sd;
+      const double sd = s, inv = 1.0 / sd;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const double e = exact(j);
-          t[j] = off_border(static_cast<float>(e * inv), e, sd);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = copysignf(off_border(mag[j] * r, mag[j], s), y[j]);
+      for (int j = 0; j < 8; ++j) {
+        const double e = exact(j);
+        t[j] = off_border(static_cast<float>(e * inv), e, sd);
       }
       code[0] = codes4(t[0], t[1], t[2], t[3]);
       code[1] = codes4(t[4], t[5], t[6], t[7]);
     }
-    uint8_t* q = p.q + row * p.ld_q + c;
-    if (vec && n == 8) {
-      *reinterpret_cast<uint2*>(q) = make_uint2(code[0], code[1]);
-    } else {
-      for (int j = 0; j < n; ++j) q[j] = static_cast<uint8_t>(code[j >> 2] >> (8 * (j & 3)));
-    }
+    store_codes(p, row, c, n, code[0], code[1]);
     if ((lane & (LANES - 1)) == 0) p.scales[row * p.ld_scales + c / GROUP] = s;
   }
 }

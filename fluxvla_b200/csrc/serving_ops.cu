@@ -69,12 +69,12 @@ int launch_norm_fp8(const fvb::n8::Dev& d, int rows, cudaStream_t st) {
   namespace N = fvb::n8;
   if (d.mode == FVB_NORM_ADA_RMS) return launch_norm_rows<TX, DT, N::SHIFT>(d, rows, st);
   if (d.mode != FVB_NORM_NONE) return launch_norm_rows<TX, DT, N::SCALE>(d, rows, st);
-  // no row statistics: runs of 2048 columns, each its own CTA.  (One vector a
-  // thread: 848 x 16384 takes 14.7 us, with two 17.8, with four 22.6, whose
-  // registers leave fewer warps to cover the latencies.)
-  const int chunks = (d.dim + N::VEC - 1) / N::VEC;
+  // no row statistics: runs of 4096 columns, each its own CTA.  (Two vectors a
+  // thread: 848 x 16384 takes 10.5 us, with one 12.4, whose maxima and scales
+  // serve half the columns, with four 12.4, whose registers leave fewer warps.)
+  const int chunks = (d.dim + 2 * N::VEC - 1) / (2 * N::VEC);
   const int t = chunks < 256 ? (chunks + 31) / 32 * 32 : 256;
-  return launch_k("fvb_norm_fp8", N::norm_fp8_kernel<TX, DT, 1, N::CODES>,
+  return launch_k("fvb_norm_fp8", N::norm_fp8_kernel<TX, DT, 2, N::CODES>,
                   dim3(rows, (chunks + t - 1) / t), dim3(t), 0, st, d);
 }
 
@@ -245,7 +245,7 @@ int fvb_norm_fp8(const fvb_norm_fp8_args* a, void* stream) {
   if (a->mode != FVB_NORM_NONE && a->dim > FVB_NORM_FP8_MAX_DIM)
     return fail(FVB_ERR_UNSUPPORTED, "fvb_norm_fp8: dim %d over %d", a->dim,
                 FVB_NORM_FP8_MAX_DIM);
-  // without one, 2^11 columns to a CTA and 2^16 - 1 CTAs to a row
+  // without one, within what 2^16 - 1 CTAs of 4096 columns cover
   if (a->dim > 65535 * 2048)
     return fail(FVB_ERR_UNSUPPORTED, "fvb_norm_fp8: dim %d over %d", a->dim, 65535 * 2048);
   if (!a->x || !a->q || !a->scales)

@@ -117,6 +117,45 @@ def test_norm_fp8_values_on_the_borders_between_codes():
         check_norm('none', row, {}, q, s)
 
 
+def test_norm_fp8_codes_of_every_bf16_quotient():
+    """Every significand of a value under every one of the group's largest, over
+    the exponents that the codes reach."""
+    m = (128 + torch.arange(128, device=DEV)).double()
+    rows = []
+    for e in range(0, 19):
+        body = (m * 2.0 ** -e).expand(128, 128).clone()
+        body[:, 1::2] *= -1
+        body = body.clamp(-m[:, None], m[:, None])
+        body[:, 0] = m
+        rows.append(body)
+    x = torch.cat(rows).to(BF16)
+    q = torch.empty(x.shape, dtype=E4M3, device=DEV)
+    s = torch.empty(x.shape[0], 1, device=DEV)
+    ops.norm_fp8(_lib.NORM_NONE, x, q, s)
+    check_norm('none', x, {}, q, s)
+
+
+@pytest.mark.parametrize('size', [1.0, 2.0 ** -40, 2.0 ** 100])
+def test_norm_fp8_codes_near_borders_of_any_scale(size):
+    """32-bit values at most three steps from a border times the scale."""
+    g = gen(15)
+    grid = R.e4m3_grid().to(DEV)
+    grid = grid[grid >= 0]
+    mid = ((grid[1:] + grid[:-1]) / 2)[:126]
+    top = (1 + torch.rand(2000, generator=g, device=DEV)) * size
+    s_ref = (top.double() / 448).float()
+    y = (mid * s_ref.double()[:, None]).float()
+    steps = torch.randint(-3, 4, y.shape, generator=g, device=DEV, dtype=torch.int32)
+    y = (y.view(torch.int32) + steps).view(F32)
+    x = torch.zeros(2000, 128, device=DEV)
+    x[:, 1:1 + y.shape[1]] = y.clamp(max=top[:, None])
+    x[:, 0] = -top
+    q = torch.empty(x.shape, dtype=E4M3, device=DEV)
+    s = torch.empty(2000, 1, device=DEV)
+    ops.norm_fp8(_lib.NORM_NONE, x, q, s)
+    check_norm('none', x, {}, q, s)
+
+
 def test_norm_fp8_zero_tiny_nan_and_infinite_rows():
     x = torch.zeros(5, 256, device=DEV)
     x[1] = 1e-30                      # below the smallest scale
