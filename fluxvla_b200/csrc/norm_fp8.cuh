@@ -142,6 +142,11 @@ __device__ __forceinline__ f32x2 pair(float a, float b) {
 __device__ __forceinline__ void unpair(f32x2 v, float& a, float& b) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
 }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
   f32x2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -310,12 +315,17 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
       load8(p.mod + p.dim + c, n, vec, b);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      y[j] = h[v][j] * rf * (1.f + w[j]);
+    for (int j = 0; j < 8; j += 2) {
+      const f32x2 one = pair(1.f, 1.f);
+      const f32x2 z = mul2(mul2(pair(h[v][j], h[v][j + 1]), pair(rf, rf)),
+                           add2(pair(w[j], w[j + 1]), one));
+      unpair(z, y[j], y[j + 1]);
       mag[j] = fabsf(y[j]);
+      mag[j + 1] = fabsf(y[j + 1]);
       if (ADA) {
-        mag[j] += fabsf(b[j]);
-        y[j] += b[j];
+        unpair(add2(pair(mag[j], mag[j + 1]), pair(fabsf(b[j]), fabsf(b[j + 1]))), mag[j],
+               mag[j + 1]);
+        unpair(add2(z, pair(b[j], b[j + 1])), y[j], y[j + 1]);
       }
     }
     auto exact = [&](int j) {
@@ -326,14 +336,22 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
     // of the values that may be the largest, the largest scale
     float low = 0.f, high = 0.f;  // fmax drops NaN: the others keep their codes
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float a = fabsf(y[j]);
-      low = fmaxf(low, ADA ? fmaf(-EPS, mag[j], a) : a);
-      high = fmaxf(high, ADA ? fmaf(EPS, mag[j], a) : a);
+    for (int j = 0; j < 8; j += 2) {
+      const float a0 = fabsf(y[j]), a1 = fabsf(y[j + 1]);
+      if (ADA) {
+        const f32x2 a = pair(a0, a1), m = pair(mag[j], mag[j + 1]);
+        float t0, t1;
+        unpair(fma2(pair(-EPS, -EPS), m, a), t0, t1);
+        low = fmaxf(low, fmaxf(t0, t1));
+        unpair(fma2(pair(EPS, EPS), m, a), t0, t1);
+        high = fmaxf(high, fmaxf(t0, t1));
+      } else {
+        low = fmaxf(low, fmaxf(a0, a1));
+      }
     }
     if (!ADA) {
+      high = low * (1.f + EPS);
       low *= 1.f - EPS;
-      high *= 1.f + EPS;
     }
     low = group_max(low);
     float s = static_cast<float>(MIN_AMAX / E4M3_MAX);
@@ -346,12 +364,15 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
     s = group_max(s);
     if (n <= 0) continue;
     // codes of both ends of each value's interval
-    const float r = rcp(s), r_lo = r * (1.f - EPS), r_hi = r * (1.f + EPS);
+    const float r = rcp(s), r_lo = ADA ? r : r * (1.f - EPS), r_hi = ADA ? r : r * (1.f + EPS);
     float lo[8], hi[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      lo[j] = ADA ? fmaf(-EPS, mag[j], y[j]) * r : y[j] * r_lo;
-      hi[j] = ADA ? fmaf(EPS, mag[j], y[j]) * r : y[j] * r_hi;
+    for (int j = 0; j < 8; j += 2) {
+      const f32x2 a = pair(y[j], y[j + 1]), m = pair(mag[j], mag[j + 1]);
+      const f32x2 below = ADA ? fma2(pair(-EPS, -EPS), m, a) : a;
+      const f32x2 above = ADA ? fma2(pair(EPS, EPS), m, a) : a;
+      unpair(mul2(below, pair(r_lo, r_lo)), lo[j], lo[j + 1]);
+      unpair(mul2(above, pair(r_hi, r_hi)), hi[j], hi[j + 1]);
     }
     uint32_t code[2] = {codes4(lo[0], lo[1], lo[2], lo[3]), codes4(lo[4], lo[5], lo[6], lo[7])};
     if (!fine || code[0] != codes4(hi[0], hi[1], hi[2], hi[3]) ||
