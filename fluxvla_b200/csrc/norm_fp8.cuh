@@ -54,56 +54,122 @@ struct Dev {
   long long ld_scales;
   int dim;
   double eps, inv_dim;
-  int vec;  // 16-byte rows everywhere: vector loads and stores
 };
 
-__device__ __forceinline__ void load8(const float* p, int n, bool vec, float (&v)[8]) {
-  if (vec && n == 8) {
-    const float4 a = *reinterpret_cast<const float4*>(p);
-    const float4 b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void from_f32(float* p, float v) { *p = v; }
+__device__ __forceinline__ void from_f32(bf16* p, float v) { *p = __float2bfloat16(v); }
+
+__device__ __forceinline__ void load_vec(const float* p, float (&v)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p);
+  const float4 b = *reinterpret_cast<const float4*>(p + 4);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load_vec(const bf16* p, float (&v)[8]) {
+  const uint4 a = *reinterpret_cast<const uint4*>(p);
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&a);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : 0.f;
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __bfloat1622float2(h[j]);
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
   }
 }
-__device__ __forceinline__ void load8(const bf16* p, int n, bool vec, float (&v)[8]) {
-  if (vec && n == 8) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&a);
+__device__ __forceinline__ void store_vec(float* p, const float (&v)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store_vec(bf16* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                            pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
+// How a warp's lanes reach their columns c..c+7 of a row, c STRIDE apart from
+// lane to lane: with 16-byte accesses where all rows allow them (VECS), else
+// with neighbouring lanes on neighbouring columns and an exchange through
+// shared memory (lanes on 8 columns each, value by value, took 71 us instead
+// of 22 on 4096 x 2047 codes of bf16 + bf16, 49 instead of 36 with an adaRMS
+// norm; only the RMS norm without a delta gains nothing, 20.6 and 22.9).  All lanes call.
+template <int STRIDE, bool VECS>
+struct Columns {
+  int dim, lane;
+  float* stage;  // [256]
+
+  // column of value lane of the warp's 256; value lane + 32 k is 4 k lanes on
+  __device__ __forceinline__ int first(int c) const {
+    return c + ((lane >> 3) - lane) * STRIDE + (lane & 7);
+  }
+  // ALIGNED: the row starts on 16 bytes
+  template <bool ALIGNED = VECS, typename T>
+  __device__ __forceinline__ void load(const T* row, int c, float (&v)[8]) const {
+    if (ALIGNED && c + 8 <= dim) {
+      load_vec(row + c, v);
+    } else if (ALIGNED) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = __bfloat1622float2(h[j]);
-      v[2 * j] = f.x;
-      v[2 * j + 1] = f.y;
+      for (int j = 0; j < 8; ++j) v[j] = c + j < dim ? to_f32(row[c + j]) : 0.f;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int at = first(c) + 4 * STRIDE * k;
+        v[k] = at < dim ? to_f32(row[at]) : 0.f;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) stage[lane + 32 * k] = v[k];
+      __syncwarp();
+      load_vec(stage + lane * 8, v);
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? __bfloat162float(p[j]) : 0.f;
   }
-}
-__device__ __forceinline__ void store8(float* p, int n, bool vec, const float (&v)[8]) {
-  if (vec && n == 8) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = v[j];
+  // of a vector that all rows share, aligned or not
+  template <typename T>
+  __device__ __forceinline__ void load_shared(const T* row, int c, float (&v)[8]) const {
+    if (VECS || (reinterpret_cast<uintptr_t>(row) & 15) == 0)
+      load<true>(row, c, v);
+    else
+      load<false>(row, c, v);
   }
-}
-__device__ __forceinline__ void store8(bf16* p, int n, bool vec, const float (&v)[8]) {
-  if (vec && n == 8) {
-    *reinterpret_cast<uint4*>(p) =
-        make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                   pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-  } else {
+  template <typename T>
+  __device__ __forceinline__ void store(T* row, int c, const float (&v)[8]) const {
+    if (VECS && c + 8 <= dim) {
+      store_vec(row + c, v);
+    } else if (VECS) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = __float2bfloat16(v[j]);
+      for (int j = 0; j < 8; ++j)
+        if (c + j < dim) from_f32(row + c + j, v[j]);
+    } else {
+      __syncwarp();
+      store_vec(stage + lane * 8, v);
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int at = first(c) + 4 * STRIDE * k;
+        if (at < dim) from_f32(row + at, stage[lane + 32 * k]);
+      }
+    }
   }
-}
+  __device__ __forceinline__ void store_codes(uint8_t* row, int c, uint32_t lo, uint32_t hi) const {
+    if (VECS && c + 8 <= dim) {
+      *reinterpret_cast<uint2*>(row + c) = make_uint2(lo, hi);
+    } else if (VECS) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < dim) row[c + j] = static_cast<uint8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
+    } else {
+      uint8_t* bytes = reinterpret_cast<uint8_t*>(stage);
+      __syncwarp();
+      *reinterpret_cast<uint2*>(bytes + lane * 8) = make_uint2(lo, hi);
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int at = first(c) + 4 * STRIDE * k;
+        if (at < dim) row[at] = bytes[lane + 32 * k];
+      }
+    }
+  }
+};
+
 // the value as the residual stream stores it
 __device__ __forceinline__ float as_stored(float v, const float*) { return v; }
 __device__ __forceinline__ float as_stored(float v, const bf16*) {
@@ -193,30 +259,22 @@ __device__ __forceinline__ float group_max(float v) {
   return v;
 }
 
-// the first n of 8 codes to columns c.. of a row
-__device__ __forceinline__ void store_codes(const Dev& p, long long row, int c, int n, uint32_t lo,
-                                            uint32_t hi) {
-  uint8_t* q = p.q + row * p.ld_q + c;
-  if (p.vec && n == 8) {
-    *reinterpret_cast<uint2*>(q) = make_uint2(lo, hi);
-  } else {
-    for (int j = 0; j < n; ++j) q[j] = static_cast<uint8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
-  }
-}
-
 // One row (or, without a norm, one run of columns of a row) per CTA; thread t
 // holds VPT vectors of 8 columns.  With a norm these are T vectors apart and 16
 // neighbouring lanes share a scale; without one they are neighbours, and 16 /
 // VPT lanes do.
-template <typename TX, int DT, int VPT, int KIND>
-__global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_kernel(const Dev p) {
+template <typename TX, int DT, int VPT, int KIND, bool VECS>
+__global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS,
+                                  KIND != CODES && VPT == 1 && !VECS ? 2 : 0)
+    norm_fp8_kernel(const Dev p) {
   constexpr bool NORM = KIND != CODES, ADA = KIND == SHIFT;
   __shared__ double part[MAX_THREADS / 32];
   const int T = blockDim.x, tid = threadIdx.x, lane = tid & 31;
   const long long row = blockIdx.x;
   const int c0 = (blockIdx.y * T + tid) * VEC * (NORM ? 1 : VPT);
   const int step = NORM ? T * VEC : VEC;  // from a thread's vector to its next
-  const bool vec = p.vec;
+  extern __shared__ __align__(16) float stage[];  // 256 a warp, if !VECS
+  const Columns<NORM ? VEC : VEC * VPT, VECS> io = {p.dim, lane, stage + (tid >> 5) * 256};
   const TX* x = static_cast<const TX*>(p.x) + row * p.ld_x;
   griddep_wait();
   griddep_launch_dependents();
@@ -224,21 +282,20 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     const int c = c0 + v * step;
-    load8(x + c, min(max(p.dim - c, 0), VEC), vec, h[v]);
+    io.load(x, c, h[v]);
   }
   if (DT != DELTA_NONE) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int c = c0 + v * step;
-      const int n = min(max(p.dim - c, 0), VEC);
       float d[8];
       if (DT == DELTA_F32)
-        load8(static_cast<const float*>(p.delta) + row * p.ld_delta + c, n, vec, d);
+        io.load(static_cast<const float*>(p.delta) + row * p.ld_delta, c, d);
       else
-        load8(static_cast<const bf16*>(p.delta) + row * p.ld_delta + c, n, vec, d);
+        io.load(static_cast<const bf16*>(p.delta) + row * p.ld_delta, c, d);
 #pragma unroll
       for (int j = 0; j < 8; ++j) h[v][j] = as_stored(h[v][j] + d[j], x);
-      store8(static_cast<TX*>(p.res) + row * p.ld_res + c, n, vec, h[v]);
+      io.store(static_cast<TX*>(p.res) + row * p.ld_res, c, h[v]);
     }
   }
   if (!NORM) {
@@ -268,8 +325,8 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) t[j] = copysignf(t[j], h[v][j]);
-      store_codes(p, row, c, min(p.dim - c, VEC), codes4(t[0], t[1], t[2], t[3]),
-                  codes4(t[4], t[5], t[6], t[7]));
+      io.store_codes(p.q + row * p.ld_q, c, codes4(t[0], t[1], t[2], t[3]),
+                     codes4(t[4], t[5], t[6], t[7]));
     }
     if ((lane & (LANES / VPT - 1)) == 0 && c0 < p.dim)
       p.scales[row * p.ld_scales + c0 / GROUP] = s;
@@ -300,19 +357,18 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     const int c = c0 + v * step;
-    const int n = min(max(p.dim - c, 0), VEC);
     // y to 32 bits, and what bounds its error: EPS * mag
     float y[8], mag[8], w[8], b[8];
     if (KIND == SCALE) {
       if (p.mode == FVB_NORM_GEMMA_RMS) {
-        load8(p.w + c, n, vec, w);
+        io.load_shared(p.w, c, w);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) w[j] = 0.f;
       }
     } else if (ADA) {
-      load8(p.mod + c, n, vec, w);
-      load8(p.mod + p.dim + c, n, vec, b);
+      io.load_shared(p.mod, c, w);
+      io.load_shared(p.mod + p.dim, c, b);
     }
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
@@ -362,7 +418,6 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
           s = fmaxf(s, static_cast<float>(fabs(exact(j)) * (1.0 / E4M3_MAX)));
     }
     s = group_max(s);
-    if (n <= 0) continue;
     // codes of both ends of each value's interval
     const float r = rcp(s), r_lo = ADA ? r : r * (1.f - EPS), r_hi = ADA ? r : r * (1.f + EPS);
     float lo[8], hi[8];
@@ -387,8 +442,8 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS) norm_fp8_ke
       code[0] = codes4(t[0], t[1], t[2], t[3]);
       code[1] = codes4(t[4], t[5], t[6], t[7]);
     }
-    store_codes(p, row, c, n, code[0], code[1]);
-    if ((lane & (LANES - 1)) == 0) p.scales[row * p.ld_scales + c / GROUP] = s;
+    io.store_codes(p.q + row * p.ld_q, c, code[0], code[1]);
+    if ((lane & (LANES - 1)) == 0 && c < p.dim) p.scales[row * p.ld_scales + c / GROUP] = s;
   }
 }
 

@@ -52,38 +52,38 @@ int make_map_u8(CUtensorMap* m, const void* ptr, int64_t rows, int64_t k, int64_
   return FVB_OK;
 }
 
-template <typename TX, int DT, int KIND>
+template <typename TX, int DT, int KIND, bool VECS>
 int launch_norm_rows(const fvb::n8::Dev& d, int rows, cudaStream_t st) {
   namespace N = fvb::n8;
   const int chunks = (d.dim + N::VEC - 1) / N::VEC;
   const int vpt = chunks <= N::MAX_THREADS ? 1 : (chunks <= 2 * N::MAX_THREADS ? 2 : 4);
   const int t = ((chunks + vpt - 1) / vpt + 31) / 32 * 32;
-  auto kern = vpt == 1   ? N::norm_fp8_kernel<TX, DT, 1, KIND>
-              : vpt == 2 ? N::norm_fp8_kernel<TX, DT, 2, KIND>
-                         : N::norm_fp8_kernel<TX, DT, 4, KIND>;
-  return launch_k("fvb_norm_fp8", kern, dim3(rows), dim3(t), 0, st, d);
+  auto kern = vpt == 1   ? N::norm_fp8_kernel<TX, DT, 1, KIND, VECS>
+              : vpt == 2 ? N::norm_fp8_kernel<TX, DT, 2, KIND, VECS>
+                         : N::norm_fp8_kernel<TX, DT, 4, KIND, VECS>;
+  return launch_k("fvb_norm_fp8", kern, dim3(rows), dim3(t), VECS ? 0 : t * 32, st, d);
 }
 
-template <typename TX, int DT>
+template <typename TX, int DT, bool VECS>
 int launch_norm_fp8(const fvb::n8::Dev& d, int rows, cudaStream_t st) {
   namespace N = fvb::n8;
-  if (d.mode == FVB_NORM_ADA_RMS) return launch_norm_rows<TX, DT, N::SHIFT>(d, rows, st);
-  if (d.mode != FVB_NORM_NONE) return launch_norm_rows<TX, DT, N::SCALE>(d, rows, st);
+  if (d.mode == FVB_NORM_ADA_RMS) return launch_norm_rows<TX, DT, N::SHIFT, VECS>(d, rows, st);
+  if (d.mode != FVB_NORM_NONE) return launch_norm_rows<TX, DT, N::SCALE, VECS>(d, rows, st);
   // no row statistics: runs of 4096 columns, each its own CTA.  (Two vectors a
   // thread: 848 x 16384 takes 10.5 us, with one 12.4, whose maxima and scales
   // serve half the columns, with four 12.4, whose registers leave fewer warps.)
   const int chunks = (d.dim + 2 * N::VEC - 1) / (2 * N::VEC);
   const int t = chunks < 256 ? (chunks + 31) / 32 * 32 : 256;
-  return launch_k("fvb_norm_fp8", N::norm_fp8_kernel<TX, DT, 2, N::CODES>,
-                  dim3(rows, (chunks + t - 1) / t), dim3(t), 0, st, d);
+  return launch_k("fvb_norm_fp8", N::norm_fp8_kernel<TX, DT, 2, N::CODES, VECS>,
+                  dim3(rows, (chunks + t - 1) / t), dim3(t), VECS ? 0 : t * 32, st, d);
 }
 
-template <typename TX>
+template <typename TX, bool VECS>
 int launch_norm_fp8(const fvb::n8::Dev& d, int delta, int rows, cudaStream_t st) {
   namespace N = fvb::n8;
-  if (delta == N::DELTA_NONE) return launch_norm_fp8<TX, N::DELTA_NONE>(d, rows, st);
-  if (delta == N::DELTA_F32) return launch_norm_fp8<TX, N::DELTA_F32>(d, rows, st);
-  return launch_norm_fp8<TX, N::DELTA_BF16>(d, rows, st);
+  if (delta == N::DELTA_NONE) return launch_norm_fp8<TX, N::DELTA_NONE, VECS>(d, rows, st);
+  if (delta == N::DELTA_F32) return launch_norm_fp8<TX, N::DELTA_F32, VECS>(d, rows, st);
+  return launch_norm_fp8<TX, N::DELTA_BF16, VECS>(d, rows, st);
 }
 
 int launch_gemm_fp8(const void* kern, const CUtensorMap& ma, const CUtensorMap& mb,
@@ -274,15 +274,20 @@ int fvb_norm_fp8(const fvb_norm_fp8_args* a, void* stream) {
   d.q = (uint8_t*)a->q; d.ld_q = a->ld_q;
   d.scales = a->scales; d.ld_scales = a->ld_scales;
   d.dim = a->dim; d.eps = a->eps; d.inv_dim = 1.0 / a->dim;
-  d.vec = rows16(a->x, a->ld_x, xb) && aligned(a->q, 8) && a->ld_q % 8 == 0 &&
-          (!a->delta || (rows16(a->delta, a->ld_delta, db) && rows16(a->res, a->ld_res, xb))) &&
-          (a->mode != FVB_NORM_GEMMA_RMS || aligned16(a->w)) &&
-          (a->mode != FVB_NORM_ADA_RMS || (aligned16(a->mod) && a->dim % 4 == 0));
+  // vector accesses where every row starts on 16 bytes (8 of the codes)
+  const bool vec =
+      rows16(a->x, a->ld_x, xb) && aligned(a->q, 8) && a->ld_q % 8 == 0 &&
+      (!a->delta || (rows16(a->delta, a->ld_delta, db) && rows16(a->res, a->ld_res, xb))) &&
+      (a->mode != FVB_NORM_GEMMA_RMS || aligned16(a->w)) &&
+      (a->mode != FVB_NORM_ADA_RMS || (aligned16(a->mod) && a->dim % 4 == 0));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int delta = !a->delta ? fvb::n8::DELTA_NONE
                               : (a->delta_f32 ? fvb::n8::DELTA_F32 : fvb::n8::DELTA_BF16);
-  if (a->x_f32) return launch_norm_fp8<float>(d, delta, a->rows, st);
-  return launch_norm_fp8<bf16>(d, delta, a->rows, st);
+  if (a->x_f32)
+    return vec ? launch_norm_fp8<float, true>(d, delta, a->rows, st)
+               : launch_norm_fp8<float, false>(d, delta, a->rows, st);
+  return vec ? launch_norm_fp8<bf16, true>(d, delta, a->rows, st)
+             : launch_norm_fp8<bf16, false>(d, delta, a->rows, st);
 }
 
 int fvb_gemm_fp8(const fvb_gemm_fp8_args* a, void* stream) {

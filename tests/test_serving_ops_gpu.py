@@ -97,6 +97,29 @@ def test_norm_fp8_strides_in_place_and_beyond_the_norm_limit():
     check_norm('none', x, {}, q, s)
 
 
+@pytest.mark.parametrize('mode', list(MODES))
+@pytest.mark.parametrize('rows,dim', [(3, 8), (2, 255), (5, 1025), (3, 4099),
+                                      (2, 16383)])
+def test_norm_fp8_unaligned_rows_and_weights(mode, rows, dim):
+    """Views that start off 16 bytes, in place, weights too; what lies around
+    them stays."""
+    g = gen(dim)
+    x, kw = norm_inputs(g, rows, dim, mode, BF16, BF16)
+    if 'w' in kw:
+        kw['w'] = torch.cat([kw['w'][:1], kw['w']])[1:]
+    if 'mod' in kw:
+        kw['mod'] = torch.cat([kw['mod'][:1], kw['mod']])[1:]
+    wide = torch.full((rows, dim + 5), 3.0, dtype=BF16, device=DEV)
+    wide[:, 3:3 + dim] = x
+    wide_q = torch.full((rows, dim + 7), 7, dtype=torch.uint8, device=DEV)
+    q, s = wide_q.view(E4M3)[:, 5:5 + dim], torch.empty(rows, -(-dim // 128), device=DEV)
+    h = wide[:, 3:3 + dim]
+    ops.norm_fp8(MODES[mode], h, q, s, res=h, **kw)
+    check_norm(mode, x, kw, q, s, h)
+    assert (wide[:, :3] == 3).all() and (wide[:, 3 + dim:] == 3).all()
+    assert (wide_q[:, :5] == 7).all() and (wide_q[:, 5 + dim:] == 7).all()
+
+
 def test_norm_fp8_values_on_the_borders_between_codes():
     """Every border of the format, times a scale that is not a power of two,
     and its neighbours: the even code, and the codes on either side."""
