@@ -411,7 +411,9 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS,
     }
     low = group_max(low);
     float s = static_cast<float>(MIN_AMAX / E4M3_MAX);
-    if (!fine || (high >= low && low > 0.f)) {
+    // (low is 0 where shifts cancel all values to within their bounds: then each
+    // of them may be the largest; a high of 0 is a value of zero)
+    if (!fine || (high >= low && high > 0.f)) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (!fine || fmaf(EPS, mag[j], fabsf(y[j])) >= low)

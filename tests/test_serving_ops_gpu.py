@@ -217,6 +217,44 @@ def test_norm_fp8_at_the_ends_of_the_range(mode, size, eps):
     assert torch.equal(s, s_ref) and torch.equal(values(q), q_ref)
 
 
+def test_norm_fp8_shifts_that_cancel_the_normed_values():
+    """Groups whose values are all small against the normed values and shifts
+    that they are the sums of: whole rows, and a last group of one column."""
+    x = torch.ones(3, 300, device=DEV)
+    x[1] = 7.0
+    x[2, ::2] = -1.0
+    mod = torch.zeros(600, device=DEV)
+    mod[300:] = -1.0
+    cases = [(x, mod)]
+    g = gen(21)
+    for dim in (1, 129, 257):
+        x = randn(g, 1, dim).expand(4, dim).contiguous()
+        mod = randn(g, 2 * dim) * 0.3
+        z = x[0].double() * torch.rsqrt(x[0].double().square().mean() + 1e-6)
+        mod[-1] = -(z * (1 + mod[:dim].double()))[-1].float()
+        cases.append((x, mod))
+    for x, mod in cases:
+        rows, dim = x.shape
+        q = torch.empty(rows, dim, dtype=E4M3, device=DEV)
+        s = torch.empty(rows, -(-dim // 128), device=DEV)
+        ops.norm_fp8(_lib.NORM_ADA_RMS, x, q, s, mod=mod)
+        h, m = x.to(F64), mod.to(F64)
+        z = h / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-6) * (1 + m[:dim])
+        y = z + m[dim:]
+        # a few roundings of 64 bits, of the terms
+        err = 2.0 ** -50 * (z.abs() + m[dim:].abs())
+        for i in range(s.shape[1]):
+            c = slice(128 * i, 128 * i + 128)
+            scale = s[:, i:i + 1].to(F64)
+            top = y[:, c].abs().amax(1, keepdim=True).clamp(min=2.0 ** -60)
+            # the scale's rounding to f32
+            near = err[:, c].amax(1, keepdim=True) + 2.0 ** -24 * top
+            assert ((448 * scale - top).abs() <= near).all()
+            # half a step of e4m3 (relative 2^-4, or of the smallest step)
+            half = 2.0 ** -4 * y[:, c].abs() + 2.0 ** -10 * scale
+            assert ((values(q[:, c]) * scale - y[:, c]).abs() <= half + near).all()
+
+
 @pytest.mark.parametrize('dt', [F32, BF16])
 def test_norm_fp8_many_codes(dt):
     """Over a million values, and groups whose largest value is a multiple of 7:
