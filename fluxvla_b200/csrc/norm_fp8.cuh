@@ -352,8 +352,11 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS,
   }
   const float rf = static_cast<float>(rstd);
   // near the ends of the 32-bit range the bounds do not hold (nor where rf is
-  // NaN): such rows are computed in 64 bits throughout
-  const bool fine = rf >= 0x1p-100f && rf <= 0x1p100f;
+  // NaN): such rows are computed in 64 bits throughout, and so are vectors with
+  // a weight above 2^40.  Below it no value overflows (a normed one is at most
+  // 2^7), and what a normed value loses below 2^-126, at most 2^-150, is no
+  // more than 2^-109 after it: nothing to the lowest border, which is 2^-79.
+  const bool fine_row = rf >= 0x1p-100f && rf <= 0x1p100f;
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     const int c = c0 + v * step;
@@ -384,6 +387,13 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS,
         unpair(add2(z, pair(b[j], b[j + 1])), y[j], y[j + 1]);
       }
     }
+    bool fine = fine_row;
+    if (KIND == SHIFT || p.mode == FVB_NORM_GEMMA_RMS) {
+      float most = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(w[j]));
+      fine = fine && most <= 0x1p40f;
+    }
     auto exact = [&](int j) {
       double r = h[v][j] * rstd * (1.0 + w[j]);
       if (ADA) r += b[j];
@@ -409,7 +419,7 @@ __global__ void __launch_bounds__(KIND == CODES ? 256 : MAX_THREADS,
       high = low * (1.f + EPS);
       low *= 1.f - EPS;
     }
-    low = group_max(low);
+    low = group_max(fine ? low : 0.f);
     float s = static_cast<float>(MIN_AMAX / E4M3_MAX);
     // (low is 0 where shifts cancel all values to within their bounds: then each
     // of them may be the largest; a high of 0 is a value of zero)

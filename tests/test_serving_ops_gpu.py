@@ -255,6 +255,34 @@ def test_norm_fp8_shifts_that_cancel_the_normed_values():
             assert ((values(q[:, c]) * scale - y[:, c]).abs() <= half + near).all()
 
 
+@pytest.mark.parametrize('mode', ['gemma', 'ada'])
+@pytest.mark.parametrize('xt', [F32, BF16])
+def test_norm_fp8_weights_up_to_the_end_of_the_range(mode, xt):
+    """Values that 32 bits do not hold, though their scales and codes do: past
+    the largest, and normed ones below the smallest under large weights."""
+    g = gen(22)
+    rows, dim = 64, 640
+    x = randn(g, rows, dim)
+    size = 20 + 18.5 * torch.rand(dim, generator=g, device=DEV)
+    w = randn(g, dim).sign() * 10.0 ** size
+    w[:128] = 3e38
+    x[:, 128:256] *= 1e-42
+    w[128:256] = 1e38
+    w[512:] *= 1e-30
+    if mode == 'gemma':
+        kw = dict(w=w.to(BF16))
+    else:
+        shift = randn(g, dim) * 10.0 ** (-3 + 40 * torch.rand(dim, generator=g, device=DEV))
+        shift[128:256] = 0
+        kw = dict(mod=torch.cat([w, shift]))
+    x = x.to(xt)
+    q = torch.empty(rows, dim, dtype=E4M3, device=DEV)
+    s = torch.empty(rows, 5, device=DEV)
+    ops.norm_fp8(MODES[mode], x, q, s, **kw)
+    assert torch.isfinite(s).all()
+    check_norm(mode, x, kw, q, s)
+
+
 @pytest.mark.parametrize('dt', [F32, BF16])
 def test_norm_fp8_many_codes(dt):
     """Over a million values, and groups whose largest value is a multiple of 7:
