@@ -168,7 +168,12 @@ __device__ __forceinline__ void scale_add(float* acc, const uint32_t* r, float f
 
 // gelu(x) * up for two pairs, gelu in its tanh form as x / (1 + exp(-2u)): no
 // cancellation where the tanh nears -1.  One reciprocal serves both; the
-// exponents are capped at 2^60 so that the product of the two stays finite.
+// exponents are capped at 2^60 so that the product of the two stays finite, and
+// at the cap (x below -7.4) gelu is 0, which is closer than 2^-59 of x.  gelu
+// is formed before its product with up, since x * up may be past the range
+// where that is not.  (x t / (1 + t) with t = exp(2u) needs neither select, but
+// a register that the pair kernel does not have: 78 us against 73.5 us on 816 x
+// 32768 x 2048.)
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -180,8 +185,9 @@ __device__ __forceinline__ void geglu2(float x0, float u0, float x1, float u1, f
   const float d0 = 1.f + ex2(fminf(x0 * fmaf(C3, x0 * x0, C1), 60.f));
   const float d1 = 1.f + ex2(fminf(x1 * fmaf(C3, x1 * x1, C1), 60.f));
   const float r = __fdividef(1.f, d0 * d1);
-  y0 = x0 * u0 * (r * d1);
-  y1 = x1 * u1 * (r * d0);
+  const float s0 = r * d1, s1 = r * d0;
+  y0 = x0 * (s0 < 0x1p-59f ? 0.f : s0) * u0;
+  y1 = x1 * (s1 < 0x1p-59f ? 0.f : s1) * u1;
 }
 
 // gelu(x) * up for one pair

@@ -362,6 +362,34 @@ def test_gemm_fp8(epi, m, n, k):
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize('m,n', [(9, 64), (9, 62), (300, 130), (4096, 8192),
+                                 (4096, 8190)])
+def test_gemm_fp8_geglu_of_gates_far_from_zero(m, n):
+    """gelu is 0 far below zero, whatever it is multiplied by, and the gate
+    itself far above it."""
+    k = 16
+    size = torch.tensor([20.0, 1e3, 1e6, 1e12, 1e19, 3e19, 1e25, 1e30, 1e37],
+                        device=DEV)
+    sa = size[torch.arange(m, device=DEV) % 9][:, None].contiguous()
+    sb = torch.ones(-(-n // 128), 1, device=DEV)
+    a, b = torch.zeros(m, k, device=DEV), torch.zeros(n, k, device=DEV)
+    a[:, 0] = 1.0
+    b[1::2, 0] = torch.where(torch.arange(n // 2, device=DEV) % 2 == 0, 1.0, -4.0)
+    out = torch.full((m, n // 2), 5.0, dtype=BF16, device=DEV)
+    b[0::2, 0] = -1.0
+    ops.gemm_fp8(a.to(E4M3), sa, b.to(E4M3), sb, out, epilogue=_lib.EPI_GEGLU)
+    assert (out == 0).all()
+    b[0::2, 0] = 1.0
+    ops.gemm_fp8(a.to(E4M3), sa, b.to(E4M3), sb, out, epilogue=_lib.EPI_GEGLU)
+    # the gate, to a few roundings of 32 bits, times up
+    c = sa.to(F64) * b[:, 0].to(F64)
+    want = c[:, 0::2] * c[:, 1::2]
+    held = want.abs() < 3e38
+    err = (BF16_HALF + 2.0 ** -20) * want.abs()
+    assert ((out.to(F64) - want).abs() <= err)[held].all()
+    assert torch.isinf(out[want.abs() > 3.5e38]).all()
+
+
 def test_gemm_fp8_nan_stays_in_its_row_and_column():
     g = gen(5)
     a, sa, b, sb = gemm_inputs(g, 70, 192, 256)
