@@ -438,11 +438,14 @@ int fvb_paged_attention(const fvb_paged_attn_args* a, void* stream) {
   if (a->n_pages < 0 || a->page_size <= 0 || a->max_pages < 0 || a->ld_table < a->max_pages)
     return fail(FVB_ERR_INVALID_ARG, "fvb_paged_attention: bad cache shape");
   const int64_t max_len = (int64_t)a->max_pages * a->page_size;
-  if (max_len > INT32_MAX - 64)
+  // the kernel counts keys in 32 bits, up to the end of the last unit and of the
+  // pages that it looks up ahead (48 units)
+  constexpr int AHEAD = 64 * fvb::paged::UNIT;
+  if (max_len > INT32_MAX - AHEAD)
     return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attention: %lld keys a sequence",
                 (long long)max_len);
   // units of 128 keys over all sequences and heads are counted in 32 bits
-  if ((max_len / 128 + 1) * a->batch > INT32_MAX / (a->kv_heads * s.head_blocks))
+  if ((max_len / fvb::paged::UNIT + 1) * a->batch > INT32_MAX / (a->kv_heads * s.head_blocks))
     return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attention: %d sequences of up to %lld keys",
                 a->batch, (long long)max_len);
   const int64_t s8[] = {a->kc_page_stride, a->kc_row_stride, a->kc_head_stride,

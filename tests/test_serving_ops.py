@@ -128,6 +128,16 @@ def test_paged_attention_refusals(kw, text, code):
     refused('fvb_paged_attention', with_(attn_args(), **kw), text, code)
 
 
+@pytest.mark.parametrize('page,pages', [
+    (48, 44739241), (8, 2 ** 28 - 9), (16, 2 ** 27 - 3), (1, 2 ** 31 - 128),
+    (1, 2 ** 31 - 1), (256, 2 ** 23 - 20)])
+def test_paged_attention_tables_at_the_end_of_32_bits(page, pages):
+    """Lengths that the kernel could not round up to whole units."""
+    refused('fvb_paged_attention',
+            with_(attn_args(), batch=1, page_size=page, max_pages=pages,
+                  ld_table=pages), 'keys a sequence', _lib.FVB_ERR_UNSUPPORTED)
+
+
 def test_workspace_does_not_depend_on_batch():
     L = _lib.lib()
     sizes = set()
