@@ -444,8 +444,12 @@ int fvb_paged_attention(const fvb_paged_attn_args* a, void* stream) {
   if (max_len > INT32_MAX - AHEAD)
     return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attention: %lld keys a sequence",
                 (long long)max_len);
-  // units of 128 keys over all sequences and heads are counted in 32 bits
-  if ((max_len / fvb::paged::UNIT + 1) * a->batch > INT32_MAX / (a->kv_heads * s.head_blocks))
+  // units of 128 keys over all sequences and heads are counted in 32 bits, and
+  // so are sequences, in strides of the block and of the grid, and a row's values
+  if ((int64_t)a->heads * a->head_dim > INT32_MAX)
+    return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attention: %d heads", a->heads);
+  if (a->batch > INT32_MAX - 1024 ||
+      (max_len / fvb::paged::UNIT + 1) * a->batch > INT32_MAX / (a->kv_heads * s.head_blocks))
     return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attention: %d sequences of up to %lld keys",
                 a->batch, (long long)max_len);
   const int64_t s8[] = {a->kc_page_stride, a->kc_row_stride, a->kc_head_stride,

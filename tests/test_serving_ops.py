@@ -138,6 +138,20 @@ def test_paged_attention_tables_at_the_end_of_32_bits(page, pages):
                   ld_table=pages), 'keys a sequence', _lib.FVB_ERR_UNSUPPORTED)
 
 
+@pytest.mark.parametrize('kw', [
+    dict(batch=2 ** 31 - 1, max_pages=0), dict(batch=2 ** 31 - 300, max_pages=7),
+    dict(batch=2 ** 30, max_pages=16), dict(batch=2 ** 28, heads=8, kv_heads=8)])
+def test_paged_attention_batches_at_the_end_of_32_bits(kw):
+    refused('fvb_paged_attention', with_(attn_args(), ld_table=16, **kw),
+            'sequences of up to', _lib.FVB_ERR_UNSUPPORTED)
+
+
+def test_paged_attention_heads_at_the_end_of_32_bits():
+    refused('fvb_paged_attention',
+            with_(attn_args(), batch=1, heads=2 ** 25, head_dim=64),
+            'heads', _lib.FVB_ERR_UNSUPPORTED)
+
+
 def test_workspace_does_not_depend_on_batch():
     L = _lib.lib()
     sizes = set()
