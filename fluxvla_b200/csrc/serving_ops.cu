@@ -380,7 +380,8 @@ int fvb_paged_append(const fvb_paged_append_args* a, void* stream) {
     return fail(FVB_ERR_INVALID_ARG, "fvb_paged_append: bad shape");
   if (a->page_size <= 0 || a->n_pages < 0)
     return fail(FVB_ERR_INVALID_ARG, "fvb_paged_append: bad cache shape");
-  if (!a->k || !a->v || !a->k_cache || !a->v_cache || !a->slots)
+  // (a cache without pages has no address)
+  if (!a->k || !a->v || !a->slots || (a->n_pages > 0 && (!a->k_cache || !a->v_cache)))
     return fail(FVB_ERR_INVALID_ARG, "fvb_paged_append: NULL operand");
   if (a->heads > 0 && (!a->q || !a->q_out))
     return fail(FVB_ERR_INVALID_ARG, "fvb_paged_append: queries need q and q_out");
@@ -433,7 +434,10 @@ int fvb_paged_attention(const fvb_paged_attn_args* a, void* stream) {
   AttendShape s;
   int r = attend_prepare(a, &s);
   if (r) return r;
-  if (!a->q || !a->k_cache || !a->v_cache || !a->page_table || !a->seq_lens || !a->out)
+  // a cache without pages has no address, nor has a table without columns
+  if (!a->q || !a->seq_lens || !a->out ||
+      (a->n_pages > 0 &&
+       (!a->k_cache || !a->v_cache || (a->max_pages > 0 && !a->page_table))))
     return fail(FVB_ERR_INVALID_ARG, "fvb_paged_attention: NULL operand");
   if (a->n_pages < 0 || a->page_size <= 0 || a->max_pages < 0 || a->ld_table < a->max_pages)
     return fail(FVB_ERR_INVALID_ARG, "fvb_paged_attention: bad cache shape");
@@ -477,7 +481,8 @@ int fvb_paged_attention(const fvb_paged_attn_args* a, void* stream) {
   d.table = a->page_table; d.ld_table = a->ld_table; d.lens = a->seq_lens;
   d.batch = a->batch; d.heads = a->heads; d.kv_heads = a->kv_heads;
   d.group = a->heads / a->kv_heads; d.head_blocks = s.head_blocks;
-  // without a page no key can be read, so every length is taken as 0
+  // without a page no key can be read, so every length is taken as 0 (and
+  // neither the cache nor the table is touched)
   d.n_pages = a->n_pages; d.page_size = a->page_size;
   d.max_len = a->n_pages > 0 ? (int)max_len : 0;
   d.scale_log2 = a->scale * 1.4426950408889634f;

@@ -699,6 +699,33 @@ def test_paged_attention_bad_lengths_and_pages_are_reported():
     assert ops.device_status() == 0 and torch.equal(out, good)
 
 
+@pytest.mark.parametrize('pages,columns', [(0, 0), (0, 3), (2, 0)])
+@pytest.mark.parametrize('batch', [1, 300])
+def test_empty_caches_and_tables(pages, columns, batch):
+    """No page, no column: empty sequences as anywhere else, others reported."""
+    g = gen(26)
+    q = randn(g, batch, 2, 64, dt=BF16)
+    cache = torch.empty(pages, 16, 1, 64, dtype=BF16, device=DEV)
+    table = torch.zeros(batch, columns, dtype=torch.int32, device=DEV)
+    ws = workspace(2, 1, 64)
+    for n, status in ((0, 0), (5, _lib.FVB_ERR_INVALID_ARG)):
+        lens = torch.full((batch,), n, dtype=torch.int32, device=DEV)
+        out, lse = torch.full_like(q, 5.0), torch.zeros(batch, 2, device=DEV)
+        ops.paged_attention(q, cache, cache, table, lens, out, scale=1.0, lse=lse,
+                            workspace=ws)
+        assert (out == 0).all() and (lse == -math.inf).all()
+        assert ops.device_status(reset=True) == status
+    # padding alone, and a slot that is not there
+    k = randn(g, batch, 1, 64, dt=BF16)
+    if pages == 0:
+        for slot, status in ((-1, 0), (0, _lib.FVB_ERR_INVALID_ARG)):
+            slots = torch.full((batch,), slot, dtype=torch.int32, device=DEV)
+            got = torch.zeros_like(q)
+            ops.paged_append(q, k, k, slots, cache, cache.clone(), q_out=got)
+            assert torch.equal(got, q if slot < 0 else torch.zeros_like(q))
+            assert ops.device_status(reset=True) == status
+
+
 def test_paged_attention_offsets_beyond_32_bits():
     """Pages more than 2^32 bytes and 2^31 elements apart."""
     g = gen(13)
