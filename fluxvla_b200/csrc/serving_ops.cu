@@ -456,15 +456,19 @@ int fvb_paged_attention(const fvb_paged_attn_args* a, void* stream) {
       (max_len / fvb::paged::UNIT + 1) * a->batch > INT32_MAX / (a->kv_heads * s.head_blocks))
     return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attention: %d sequences of up to %lld keys",
                 a->batch, (long long)max_len);
-  const int64_t s8[] = {a->kc_page_stride, a->kc_row_stride, a->kc_head_stride,
-                        a->vc_page_stride, a->vc_row_stride, a->vc_head_stride};
+  // the stride of a dimension of size 1 means nothing, and is taken as 0
+  auto step = [](int64_t stride, int32_t size) { return size == 1 ? 0 : stride; };
+  const int64_t s8[] = {step(a->kc_page_stride, a->n_pages), step(a->kc_row_stride, a->page_size),
+                        step(a->kc_head_stride, a->kv_heads), step(a->vc_page_stride, a->n_pages),
+                        step(a->vc_row_stride, a->page_size), step(a->vc_head_stride, a->kv_heads)};
   bool ok = aligned16(a->k_cache) && aligned16(a->v_cache);
   for (int64_t v : s8) ok = ok && v % 8 == 0;
   if (!ok)
     return fail(FVB_ERR_INVALID_ARG,
                 "fvb_paged_attention: cache rows must be 16B aligned (strides in multiples of 8)");
-  if (!aligned(a->q, 4) || a->q_row_stride % 2 || a->q_head_stride % 2 || !aligned(a->out, 8) ||
-      a->out_row_stride % 4 || a->out_head_stride % 4)
+  const int64_t q_rs = step(a->q_row_stride, a->batch), q_hs = step(a->q_head_stride, a->heads),
+                o_rs = step(a->out_row_stride, a->batch), o_hs = step(a->out_head_stride, a->heads);
+  if (!aligned(a->q, 4) || q_rs % 2 || q_hs % 2 || !aligned(a->out, 8) || o_rs % 4 || o_hs % 4)
     return fail(FVB_ERR_INVALID_ARG,
                 "fvb_paged_attention: q needs 4-byte, out 8-byte aligned rows");
   if (!a->workspace || a->workspace_bytes < s.bytes || !aligned16(a->workspace))
@@ -473,10 +477,10 @@ int fvb_paged_attention(const fvb_paged_attn_args* a, void* stream) {
   if (a->batch == 0) return FVB_OK;
   g_used.store(true, std::memory_order_relaxed);
   fvb::paged::AttendDev d;
-  d.q = (const bf16*)a->q; d.q_rs = a->q_row_stride; d.q_hs = a->q_head_stride;
+  d.q = (const bf16*)a->q; d.q_rs = q_rs; d.q_hs = q_hs;
   d.k = (const bf16*)a->k_cache; d.k_ps = s8[0]; d.k_rs = s8[1]; d.k_hs = s8[2];
   d.v = (const bf16*)a->v_cache; d.v_ps = s8[3]; d.v_rs = s8[4]; d.v_hs = s8[5];
-  d.o = (bf16*)a->out; d.o_rs = a->out_row_stride; d.o_hs = a->out_head_stride;
+  d.o = (bf16*)a->out; d.o_rs = o_rs; d.o_hs = o_hs;
   d.lse = a->lse; d.lse_rs = a->lse_row_stride;
   d.table = a->page_table; d.ld_table = a->ld_table; d.lens = a->seq_lens;
   d.batch = a->batch; d.heads = a->heads; d.kv_heads = a->kv_heads;

@@ -435,7 +435,8 @@ typedef struct fvb_paged_attn_args {
  * the sequence's pages; query head h reads kv head h / (heads / kv_heads).
  * One launch whatever the lengths are: they are read on the device, so a
  * captured call follows them.  A length of 0 gives zeros and lse = -inf.
- * Table entries past a sequence's last page are not read.  A length outside
+ * Table entries past a sequence's last page are not read; the stride of a
+ * dimension of size 1 may be anything.  A length outside
  * [0, max_pages * page_size] is clamped, a page outside the cache read as
  * page 0, and either sets FVB_ERR_INVALID_ARG in the device status word.
  *

@@ -1,6 +1,7 @@
 """The serving operators (e4m3 norm and product, paged append and attention)
 against 64-bit restatements, at the sizes, strides and masks where they can go
 wrong; then a decoder layer of them, in order."""
+import ctypes as C
 import math
 
 import pytest
@@ -637,6 +638,33 @@ def test_single_rows_heads_and_pages_of_any_stride():
     ops.paged_attention(q4, kc4, vc4, table, ln, out, scale=0.2, lse=lse,
                         workspace=workspace(8, 4, 64))
     check_attention(out, lse, q4, kc4, vc4, table, ln, 0.2)
+
+
+@pytest.mark.parametrize('page', [16, 7, 1])
+def test_single_rows_heads_and_pages_of_any_stride_in_c(page):
+    """The same through the C entry, which is given every stride."""
+    g = gen(27)
+    pages = 1 if page > 1 else 9
+    n = page * pages
+    kc, vc = (randn(g, pages, page, 1, 64, dt=BF16) for _ in range(2))
+    q, out = randn(g, 1, 1, 64, dt=BF16), torch.empty(1, 1, 64, dtype=BF16, device=DEV)
+    table = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    ln = torch.tensor([n], dtype=torch.int32, device=DEV)
+    lse, ws = torch.empty(1, 1, device=DEV), workspace(1, 1, 64)
+    a = _lib.PagedAttnArgs(
+        q=q.data_ptr(), q_row_stride=13, q_head_stride=-5, k_cache=kc.data_ptr(),
+        kc_page_stride=page * 64 if pages > 1 else 3,
+        kc_row_stride=64 if page > 1 else 5, kc_head_stride=7,
+        v_cache=vc.data_ptr(), vc_page_stride=page * 64 if pages > 1 else -1,
+        vc_row_stride=64 if page > 1 else 1, vc_head_stride=9, n_pages=pages,
+        page_size=page, page_table=table.data_ptr(), ld_table=pages,
+        max_pages=pages, seq_lens=ln.data_ptr(), out=out.data_ptr(),
+        out_row_stride=1, out_head_stride=2, lse=lse.data_ptr(), lse_row_stride=1,
+        batch=1, heads=1, kv_heads=1, head_dim=64, scale=0.2,
+        workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+    st = torch.cuda.current_stream().cuda_stream
+    assert _lib.lib().fvb_paged_attention(C.byref(a), C.c_void_p(st)) == 0
+    check_attention(out, lse, q, kc, vc, table, ln, 0.2)
 
 
 def test_calls_on_two_streams_and_graphs_that_share_a_workspace():
