@@ -223,7 +223,8 @@ __device__ __forceinline__ void store8(const Dev& p, int t, int f, const float (
 // fac[slot][block][row][group].  Lanes run over the groups first: 16 bytes of a
 // row are one access, where a load of one group for 32 rows would touch 32
 // lines, and every summing warp would repeat it.  bt counts batches over a
-// CTA's tiles.
+// CTA's tiles.  (Ordinary loads: the kernel starts while the norm that writes sa
+// may still run, and __ldg is for data that nothing writes meanwhile.)
 template <int BLOCKS>
 __device__ __forceinline__ bool write_factors(const Dev& p, int t0, int block, int g0, int g1,
                                               float* fac, uint64_t* ffull, uint64_t* fempty,
@@ -235,10 +236,10 @@ __device__ __forceinline__ bool write_factors(const Dev& p, int t0, int block, i
     float a[16], b[BLOCKS];
 #pragma unroll
     for (int i = 0; i < BLOCKS; ++i)
-      b[i] = __ldg(p.sb + (long long)min(block + i, last) * p.ld_sb + ge);
+      b[i] = p.sb[(long long)min(block + i, last) * p.ld_sb + ge];
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      a[i] = __ldg(p.sa + (long long)min(t0 + i * 8 + r0, p.m - 1) * p.ld_sa + ge);
+      a[i] = p.sa[(long long)min(t0 + i * 8 + r0, p.m - 1) * p.ld_sa + ge];
     if (!mbar_wait(&fempty[slot], ((bt >> 1) & 1) ^ 1)) return false;
     float* f = fac + slot * (BATCH * 128 * BLOCKS);
 #pragma unroll

@@ -2,6 +2,11 @@
 // strides: rows are appended with the rotary positions applied on the way
 // (append_kernel), and one new token of each sequence attends over the pages
 // of its table row (attend_kernel).
+//
+// The kernels start while the one before them in the stream may still write
+// what they read, so everything is read by ordinary loads after griddep_wait:
+// the read-only path (__ldg) is for data that nothing writes in the kernel's
+// life, its start before that wait included.
 #pragma once
 
 #include "attention.cuh"
@@ -82,11 +87,11 @@ __device__ __forceinline__ bool row_of(const AppendDev& p, long long tok, int he
 
 // A token's slot and position; false if its rows are left alone.
 __device__ __forceinline__ bool token_of(const AppendDev& p, long long tok, int* slot, int* pos) {
-  *slot = __ldg(p.slots + tok);
+  *slot = p.slots[tok];
   *pos = 0;
   bool ok = *slot < p.n_slots;
   if (p.rope_cs) {
-    *pos = __ldg(p.positions + tok);
+    *pos = p.positions[tok];
     if (*pos < 0 || *pos >= p.max_pos) {
       if (*slot < 0) return false;  // padding has no position; a cached row needs one
       ok = false;
@@ -121,7 +126,7 @@ __global__ void __launch_bounds__(256) append_vec_kernel(const AppendDev p) {
   if (h0 < rotated) {
     const float4* t = reinterpret_cast<const float4*>(p.rope_cs + ((long long)pos * (p.dim / 2) + ch * 8) * 2);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) cs[i] = __ldg(t + i);
+    for (int i = 0; i < 4; ++i) cs[i] = t[i];
   }
   constexpr int U = 2;
   for (int hb = h0; hb < h1; hb += U) {
@@ -192,7 +197,7 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendDev p) {
   const int first = half ? ch : 2 * ch, second = half ? ch + p.dim / 2 : 2 * ch + 1;
   bf16 a = row.src[first], b = row.src[second];
   if (turn) {
-    const float2 cs = __ldg(reinterpret_cast<const float2*>(p.rope_cs) + (long long)pos * per_head + ch);
+    const float2 cs = reinterpret_cast<const float2*>(p.rope_cs)[(long long)pos * per_head + ch];
     float x = __bfloat162float(a), y = __bfloat162float(b);
     rotate(x, y, cs.x, cs.y);
     a = __float2bfloat16(x);
@@ -314,7 +319,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 __device__ __forceinline__ int clamped_len(const AttendDev& p, int b) {
-  const int n = __ldg(p.lens + b);
+  const int n = p.lens[b];
   return min(max(n, 0), p.max_len);
 }
 
@@ -441,7 +446,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   int mine = 0;
   for (int b = b_lo; b < b_hi; ++b) {
     const int n = clamped_len(p, b);
-    if (n != __ldg(p.lens + b)) record_device_error(FVB_ERR_INVALID_ARG);
+    if (n != p.lens[b]) record_device_error(FVB_ERR_INVALID_ARG);
     mine += (n + UNIT - 1) / UNIT;
   }
   int upto = mine;
@@ -530,7 +535,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int t = BOXES ? tile + lane : tile;
     const int k = (run.k_first + t) * UNIT + warp * SUB + (BOXES ? 0 : lane & (SUB - 1));
     return t < run.n_tiles && k < run.len
-               ? __ldg(p.table + run.b * p.ld_table + (unsigned)k / (unsigned)p.page_size) : 0;
+               ? p.table[run.b * p.ld_table + (unsigned)k / (unsigned)p.page_size] : 0;
   };
   auto start_pages = [&]() { pages_ahead = load_pages(0); };
   int page = 0, at = 0;  // of the tile that is requested

@@ -897,3 +897,120 @@ def test_decoder_layer_of_one_token_per_request(tokens):
     a, sa, _ = codes('none', h)
     y = x2 + product(a, sa, dn_w, dn_s, 'f32')
     assert torch.isfinite(y).all() and ops.device_status() == 0
+
+
+class Layer:
+    """The operators of a decoder layer on buffers of its own, one call after
+    the other; ``sync`` waits for the GPU after each."""
+
+    def __init__(self, tokens, seed):
+        g = gen(seed)
+        self.tokens, self.g = tokens, g
+        self.heads, self.dim, page, width, mlp = 8, 128, 16, 1024, 2048
+
+        def weight(n, k, geglu=False):
+            w = randn(g, n, k) * k ** -0.5
+            if geglu:
+                w = pack.pack_geglu(w[:n // 2], w[n // 2:])
+            return pack.quantize_blocks(w)
+
+        def codes(n):
+            return (torch.empty(tokens, n, dtype=E4M3, device=DEV),
+                    torch.empty(tokens, n // 128, device=DEV))
+
+        self.qkv_w = weight((self.heads + 2) * self.dim, width)
+        self.o_w = weight(width, self.heads * self.dim)
+        self.gu_w, self.dn_w = weight(2 * mlp, width, True), weight(width, mlp)
+        self.w1, self.w2 = (randn(g, width, dt=BF16) * 0.1 for _ in range(2))
+        lens = [(37 * i) % 500 + 1 for i in range(tokens)]
+        _, self.kc, self.vc, self.table, _ = paged_inputs(
+            g, lens, self.heads, 1, self.dim, page)
+        self.lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        self.cs = rope(512, self.dim)
+        self.x = torch.empty(tokens, width, device=DEV)
+        self.c = [codes(width), codes(self.heads * self.dim), codes(width), codes(mlp)]
+        self.qkv = torch.empty(tokens, (self.heads + 2) * self.dim, dtype=BF16, device=DEV)
+        self.q, self.att = (torch.empty(tokens, self.heads, self.dim, dtype=BF16, device=DEV)
+                            for _ in range(2))
+        self.o, self.down = (torch.empty(tokens, width, dtype=BF16, device=DEV)
+                             for _ in range(2))
+        self.h = torch.empty(tokens, mlp, dtype=BF16, device=DEV)
+        self.lse = torch.empty(tokens, self.heads, device=DEV)
+        self.ws = workspace(self.heads, 1, self.dim)
+        self.at, self.slots = torch.empty_like(self.lens), torch.empty_like(self.lens)
+
+    def inputs(self):
+        """A new residual row and a new place in the cache for each token."""
+        self.x.copy_(randn(self.g, *self.x.shape))
+        at = (torch.rand(self.tokens, generator=self.g, device=DEV) * self.lens).int()
+        rows = torch.arange(self.tokens, device=DEV)
+        self.at.copy_(at)
+        self.slots.copy_(self.table[rows, (at // 16).long()] * 16 + at % 16)
+
+    def run(self, sync=False):
+        heads, wait = self.heads, torch.cuda.synchronize if sync else lambda: None
+        rows = self.qkv.unflatten(1, (heads + 2, self.dim))
+        (a, sa), (b, sb), (c, sc), (d, sd) = self.c
+        for call in (
+                lambda: ops.norm_fp8(_lib.NORM_GEMMA_RMS, self.x, a, sa, w=self.w1),
+                lambda: ops.gemm_fp8(a, sa, *self.qkv_w, self.qkv),
+                lambda: ops.paged_append(
+                    rows[:, :heads], rows[:, heads:heads + 1], rows[:, heads + 1:],
+                    self.slots, self.kc, self.vc, q_out=self.q, positions=self.at,
+                    rope_cs=self.cs),
+                lambda: ops.paged_attention(
+                    self.q, self.kc, self.vc, self.table, self.lens, self.att,
+                    scale=self.dim ** -0.5, lse=self.lse, workspace=self.ws),
+                lambda: ops.norm_fp8(_lib.NORM_NONE, self.att.flatten(1), b, sb),
+                lambda: ops.gemm_fp8(b, sb, *self.o_w, self.o),
+                lambda: ops.norm_fp8(_lib.NORM_GEMMA_RMS, self.x, c, sc, w=self.w2,
+                                     delta=self.o, res=self.x),
+                lambda: ops.gemm_fp8(c, sc, *self.gu_w, self.h, epilogue=_lib.EPI_GEGLU),
+                lambda: ops.norm_fp8(_lib.NORM_NONE, self.h, d, sd),
+                lambda: ops.gemm_fp8(d, sd, *self.dn_w, self.down)):
+            call()
+            wait()
+
+    def state(self):
+        # bytes: the unused rows of the caches are NaN
+        return [t.clone().view(torch.uint8) for t in (
+            self.x, self.down, self.h, self.o, self.att, self.lse, self.q, self.kc, self.vc,
+            *(t for pair in self.c for t in pair))]
+
+
+@pytest.mark.parametrize('tokens', [1, 16, 200])
+def test_layers_back_to_back_equal_layers_call_by_call(tokens):
+    """Each kernel may start while the one before it still writes what it reads
+    (codes, scales, queries, cache rows): ten layers of new inputs without a
+    wait, eager and captured, against the same with a wait after every call."""
+    steps, step, eager, graphed = 10, *(Layer(tokens, 40) for _ in range(3))
+    want, got = [], []
+    for _ in range(steps):
+        step.inputs()
+        step.run(sync=True)
+        want.append(step.state())
+    torch.cuda.synchronize()
+    for _ in range(steps):
+        eager.inputs()
+        eager.run()
+        got.append(eager.state())
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    # captured: two layers in a row on the same inputs
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        graphed.run()
+        graphed.run()
+    step, twice = Layer(tokens, 40), []
+    for _ in range(steps):
+        step.inputs()
+        step.run(sync=True)
+        step.run(sync=True)
+        twice.append(step.state())
+    for a in twice:
+        graphed.inputs()
+        graph.replay()
+        assert all(torch.equal(x, y) for x, y in zip(a, graphed.state()))
+    assert ops.device_status() == 0
