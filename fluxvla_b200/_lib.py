@@ -159,6 +159,7 @@ EXPORTS = {
     'fvb_expert_trace_read': (C.c_int, [C.c_void_p, C.c_int32]),
     'fvb_gemm_trace_read': (C.c_int, [C.c_void_p, C.c_int32]),
     'fvb_get_device_status': (C.c_int, [C.POINTER(C.c_int), C.c_int]),
+    'fvb_get_model_status': (C.c_int, [C.POINTER(C.c_int), C.c_int]),
     'fvb_last_error': (C.c_char_p, []),
     'fvb_version': (C.c_int, []),
     'fvb_launch_count': (C.c_int64, []),

@@ -254,7 +254,7 @@ int fvb_version(void) { return 1; }
 const char* fvb_last_error(void) { return g_err; }
 int64_t fvb_launch_count(void) { return g_launches.load(); }
 
-int fvb_get_device_status(int* status, int reset) {
+int fvb_get_model_status(int* status, int reset) {
   if (!status) return fail(FVB_ERR_INVALID_ARG, "status is NULL");
   cudaError_t e = cudaMemcpyFromSymbol(status, g_fvb_device_status, sizeof(int));
   if (e != cudaSuccess)
@@ -265,10 +265,14 @@ int fvb_get_device_status(int* status, int reset) {
     if (e != cudaSuccess)
       return fail(FVB_ERR_CUDA, "reset status: %s", cudaGetErrorString(e));
   }
+  return FVB_OK;
+}
+
+int fvb_get_device_status(int* status, int reset) {
+  if (int r = fvb_get_model_status(status, reset)) return r;
   // the serving operators' kernels have a status word of their own
   int other = FVB_OK;
-  const int r = fvb_serving_device_status(&other, reset);
-  if (r) return r;
+  if (int r = fvb_serving_device_status(&other, reset)) return r;
   if (*status == FVB_OK) *status = other;
   return FVB_OK;
 }

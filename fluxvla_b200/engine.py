@@ -695,10 +695,11 @@ class PI0EngineB200:
         chunk's synchronisation; on an error it is cleared, the engine's
         synchronisation state (the persistent step's barrier counter and
         abort flag, split-K workspaces) is zeroed so that the next chunk
-        starts clean, and the error is raised."""
-        st = ops.device_status()
+        starts clean, and the error is raised.  What the operators for
+        several requests record is left to their callers."""
+        st = ops.device_status(serving=False)
         if st:
-            ops.device_status(reset=True)
+            ops.device_status(reset=True, serving=False)
             self.reset_sync_state()
             raise RuntimeError(
                 f'fluxvla_b200: device status {st} (a kernel wait gave up); '

@@ -123,8 +123,8 @@ class GemmaLayerB200:
                                      pin_memory=True)
         self._host.copy_(self.B['x'], non_blocking=True)
         torch.cuda.current_stream(self.dev).synchronize()
-        st = ops.device_status()
+        st = ops.device_status(serving=False)
         if st:
-            ops.device_status(reset=True)
+            ops.device_status(reset=True, serving=False)
             raise RuntimeError(f'fluxvla_b200: device status {st}')
         return self._host.clone().reshape(1, self.S, -1)

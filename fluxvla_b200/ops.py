@@ -269,9 +269,14 @@ def probe_wait_timeout(limit_s: float = 0.05) -> bool:
     return g.value == 1
 
 
-def device_status(reset: bool = False) -> int:
+def device_status(reset: bool = False, *, serving: bool = True) -> int:
+    """What kernels on the current device have recorded since the last reset
+    (0 or an FVB_ERR_* code).  ``serving=False`` leaves the operators for
+    several requests out (fvb_get_model_status), unread and unreset."""
     s = C.c_int(0)
-    check(_lib.lib().fvb_get_device_status(C.byref(s), int(reset)))
+    L = _lib.lib()
+    read = L.fvb_get_device_status if serving else L.fvb_get_model_status
+    check(read(C.byref(s), int(reset)))
     return s.value
 
 

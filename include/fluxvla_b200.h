@@ -527,8 +527,13 @@ int fvb_gemm_trace_read(uint64_t* host_out, int32_t max_ctas);
  * for layer 0, the end of each phase's work and of its grid barrier. */
 int fvb_expert_trace_read(uint64_t* host_out, int32_t max_ctas);
 
-/* Status and diagnostics. */
+/* Status and diagnostics: what kernels on the current device have recorded
+ * since the last reset.  fvb_get_device_status covers all kernels,
+ * fvb_get_model_status all but those of the operators for several requests
+ * (fvb_norm_fp8, fvb_gemm_fp8, fvb_paged_*): what those record, a slot outside
+ * the cache for instance, is no failure of a model that runs beside them.   */
 int fvb_get_device_status(int* status, int reset);
+int fvb_get_model_status(int* status, int reset);
 
 /* Failure-path self test (no reference counterpart): launches one thread
  * that waits, through the library's bounded mbarrier wait, on a barrier

@@ -157,6 +157,37 @@ def test_stale_abort_flag_is_reported_and_cleared():
     assert (again - clean).abs().max().item() < 1e-2
 
 
+def test_a_bad_slot_of_another_request_is_no_failure_of_the_engine():
+    """What the paged operators record stays in the status word for their
+    caller: the engine's chunks before and after are good, and the word is not
+    cleared by them."""
+    from fluxvla_b200 import _lib, ops
+    cfg = PI0Config(exp_layers=2, llm_layers=2)
+    W = make_weights(cfg, 1, parts=('exp', 'heads'))
+    E = 816
+    g = torch.Generator().manual_seed(3)
+    k = torch.randn(cfg.exp_layers, E, cfg.head_dim, generator=g).bfloat16()
+    v = torch.randn(cfg.exp_layers, E, cfg.head_dim, generator=g).bfloat16()
+    state = torch.randn(1, cfg.state_dim, generator=g)
+    noise = torch.randn(1, cfg.n_actions, cfg.action_dim, generator=g)
+    eng = PI0EngineB200(cfg, W, prefix_len=E)
+    eng.set_prefix_cache(k.cuda(), v.cuda())
+    ops.device_status(reset=True)
+    clean = eng.predict_action(states=state, noise=noise)
+    row = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device='cuda')
+    cache = torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16, device='cuda')
+    slot = torch.tensor([9], dtype=torch.int32, device='cuda')
+    ops.paged_append(None, row, row, slot, cache, cache.clone())
+    again = eng.predict_action(states=state, noise=noise)
+    assert (again - clean).abs().max().item() < 1e-2
+    assert ops.device_status(serving=False) == 0
+    _abort_word(eng).fill_(1)
+    with pytest.raises(RuntimeError, match='device status 4'):
+        eng.predict_action(states=state, noise=noise)
+    assert ops.device_status(reset=True) == _lib.FVB_ERR_INVALID_ARG
+    assert ops.device_status() == 0
+
+
 def test_config0_gemma_layer_causal_816_rows():
     """config[0]: one Gemma-2B decoder layer, x [1, 816, 2048] ~N(0,1),
     causal mask, positions 0..815, through the prefill kernels (captured
