@@ -1,11 +1,14 @@
 // Residual addition, RMS norm and e4m3 codes with one f32 scale per 128
 // columns of a row, in one pass: what an 8-bit product reads next.
 //
-//   h = round(x + delta)                     (stored as the new residual)
+//   h = x + delta                            (stored as the new residual)
 //   y = h * rsqrt(mean(h^2) + eps) * (1 + w) | * (1 + scale) + shift | h
 //   s_g = f32(max(max_g |y|, 2^-60) / 448),  q = rne_e4m3(y / s_g)
 //
-// The codes and scales are those of the formula without rounding in between:
+// The sum is formed in f32 and rounded to x's type, as (x + delta).to(x.dtype)
+// is: for bf16 x and an f32 delta that is two roundings, off by half a step and
+// 2^-17 of one at most.  From h on, the codes and scales are those of the formula
+// without rounding in between:
 // a value computed to 32 bits lands on the wrong side of a border between two
 // codes for a few elements in a million, and is then off by a whole code.  All
 // of it in 64 bits is bound by the conversions (848 x 16384 bf16 codes: 24 us

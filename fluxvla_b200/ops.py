@@ -204,8 +204,8 @@ def norm_fp8(mode: int, x: torch.Tensor, out: torch.Tensor,
              scales: torch.Tensor, *, delta=None, res=None, w=None, mod=None,
              eps: float = 1e-6) -> None:
     """e4m3 codes of normalised rows, one f32 scale per 128 columns
-    (fvb_norm_fp8): ``res`` = x + delta if ``delta`` is given (``res`` may be
-    ``x``), then NORM_GEMMA_RMS (w), NORM_ADA_RMS (mod: scale | shift),
+    (fvb_norm_fp8): ``res`` = x + delta (in f32, rounded to x's type) if
+    ``delta`` is given (``res`` may be ``x``), then NORM_GEMMA_RMS (w), NORM_ADA_RMS (mod: scale | shift),
     NORM_RMS or NORM_NONE, then ``out`` (float8_e4m3fn [rows, dim]) and
     ``scales`` ([rows, ceil(dim / 128)]).  x: f32 or bf16 rows, delta
     either."""

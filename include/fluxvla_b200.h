@@ -338,12 +338,13 @@ typedef struct fvb_norm_fp8_args {
 } fvb_norm_fp8_args;
 
 /* Residual addition, norm and e4m3 codes of rows, what fvb_gemm_fp8 reads:
- *   h = round(x + delta)           -> res (x's type; h = x without delta)
+ *   h = x + delta, added in f32    -> res (rounded to x's type; h = x
+ *                                     without delta)
  *   y = h * rsqrt(mean(h^2) + eps) * (1 + w) | * (1 + scale) + shift | h
  *   scale of 128 columns = max(max |y|, 2^-60) / 448, rounded to f32
  *   code = y / scale rounded to e4m3 (ties to even)
- * Between its inputs and the two roundings nothing is rounded to fewer than
- * 64 bits.  A NaN gets the NaN code and does not count for its group's
+ * Between h and the last two roundings nothing is rounded to fewer than 64
+ * bits.  A NaN gets the NaN code and does not count for its group's
  * scale; a group that holds an infinity has an infinite scale and decodes as
  * NaN.  rows = 0 is a call that does nothing.  Rows that are 16-byte aligned
  * (x, delta, res) and 8-byte aligned (q) are moved in vectors, others value by

@@ -121,6 +121,23 @@ def test_norm_fp8_unaligned_rows_and_weights(mode, rows, dim):
     assert (wide_q[:, :5] == 7).all() and (wide_q[:, 5 + dim:] == 7).all()
 
 
+@pytest.mark.parametrize('dim', [128, 131])
+def test_norm_fp8_sum_is_formed_in_f32(dim):
+    """1 + 2^-8 + 2^-31 is 1 + 2^-8 in f32, which goes to the even bf16, 1."""
+    g = gen(28)
+    x = torch.ones(64, dim, dtype=BF16, device=DEV)
+    delta = 2.0 ** -8 + randn(g, 64, dim) * 2.0 ** -31
+    delta[0] = 2.0 ** -8 + 2.0 ** -31
+    for x, delta in ((x, delta), (randn(g, 64, dim, dt=BF16), randn(g, 64, dim)),
+                     (randn(g, 64, dim), randn(g, 64, dim, dt=BF16))):
+        res = torch.empty_like(x)
+        q = torch.empty(64, dim, dtype=E4M3, device=DEV)
+        s = torch.empty(64, -(-dim // 128), device=DEV)
+        ops.norm_fp8(_lib.NORM_NONE, x, q, s, delta=delta, res=res)
+        assert torch.equal(res, (x.float() + delta.float()).to(x.dtype))
+        check_norm('none', res, {}, q, s)
+
+
 def test_norm_fp8_values_on_the_borders_between_codes():
     """Every border of the format, times a scale that is not a power of two,
     and its neighbours: the even code, and the codes on either side."""
