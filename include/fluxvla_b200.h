@@ -344,9 +344,10 @@ typedef struct fvb_norm_fp8_args {
  *   scale of 128 columns = max(max |y|, 2^-60) / 448, rounded to f32
  *   code = y / scale rounded to e4m3 (ties to even)
  * Between h and the last two roundings nothing is rounded to fewer than 64
- * bits.  A NaN gets the NaN code and does not count for its group's
- * scale; a group that holds an infinity has an infinite scale and decodes as
- * NaN.  rows = 0 is a call that does nothing.  Rows that are 16-byte aligned
+ * bits.  A NaN among the y gets the NaN code and does not count for its
+ * group's scale; a group that holds an infinity has an infinite scale and
+ * decodes as NaN.  (An infinity in x is a NaN among the y of its row, whose
+ * others are 0 or the shift; a NaN in x makes the whole row NaN.)  rows = 0 is a call that does nothing.  Rows that are 16-byte aligned
  * (x, delta, res) and 8-byte aligned (q) are moved in vectors, others value by
  * value.                                                                    */
 int fvb_norm_fp8(const fvb_norm_fp8_args* args, void* stream);
@@ -368,7 +369,9 @@ typedef struct fvb_gemm_fp8_args {
 
 /* out[t, f] = sum over groups g of 128 columns of a_scale[t, g] *
  * b_scale[f / 128, g] * (sum over k in g of a[t, k] * b[f, k]), accumulated
- * in f32; GEGLU as in fvb_gemm (features 2i, 2i+1 are gate and up of output
+ * in f32, the two scales multiplied first (so their product has to be within
+ * f32's range); NaN codes and infinite scales make their row or column NaN,
+ * and no other.  GEGLU as in fvb_gemm (features 2i, 2i+1 are gate and up of output
  * i).  k need not be a multiple of 128.  The sums have a fixed order: the same
  * call gives the same bits.  m = 0 is a call that does nothing.             */
 int fvb_gemm_fp8(const fvb_gemm_fp8_args* args, void* stream);
@@ -440,6 +443,14 @@ typedef struct fvb_paged_attn_args {
  * dimension of size 1 may be anything.  A length outside
  * [0, max_pages * page_size] is clamped, a page outside the cache read as
  * page 0, and either sets FVB_ERR_INVALID_ARG in the device status word.
+ *
+ * Scores and sums are formed in f32.  A head whose scores are all -infinity
+ * gives zeros and lse = -inf too (the formula has no value there).  A NaN in a
+ * query or a key, or a score of +infinity, makes the head's output and lse NaN;
+ * an infinite or NaN value makes its dimension of the outputs infinite or NaN
+ * (weights are applied in two halves, whose products with an infinity may
+ * differ in sign).  Nothing else is affected, and cache rows past a sequence's
+ * length may hold anything.
  *
  * The workspace must be zero-filled before its first use and every call
  * leaves it ready for the next, of any shape (after FVB_ERR_DEVICE_TIMEOUT it

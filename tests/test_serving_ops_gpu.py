@@ -301,6 +301,33 @@ def test_norm_fp8_weights_up_to_the_end_of_the_range(mode, xt):
     check_norm(mode, x, kw, q, s)
 
 
+@pytest.mark.parametrize('mode', ['gemma', 'ada', 'rms'])
+@pytest.mark.parametrize('bad', [math.nan, math.inf, -math.inf])
+def test_norm_fp8_rows_that_are_not_finite(mode, bad):
+    g = gen(25)
+    x, kw = norm_inputs(g, 5, 300, mode, F32, None)
+    x[2, 200] = bad
+    q = torch.empty(5, 300, dtype=E4M3, device=DEV)
+    s = torch.empty(5, 3, device=DEV)
+    ops.norm_fp8(MODES[mode], x, q, s, **kw)
+    rest = torch.arange(5, device=DEV) != 2
+    check_norm(mode, x[rest], kw, q[rest], s[rest])
+    v = values(q[2]) * s[2].to(F64).repeat_interleave(128)[:300]
+    others = torch.arange(300, device=DEV) != 200
+    assert torch.isnan(v[200])
+    if bad != bad:
+        assert torch.isnan(v).all()
+    elif mode == 'ada':
+        # the shift, to half a step (or half the smallest step of its group)
+        shift = kw['mod'][300:].to(F64)
+        top = torch.nn.functional.pad(shift.abs(), (0, 84)).view(3, 128).amax(1)
+        low = top.repeat_interleave(128)[:300] / 448 * 2.0 ** -10
+        err = (v - shift).abs() - (2.0 ** -4 * shift.abs() + low) * (1 + 2.0 ** -20)
+        assert (err[others] <= 0).all()
+    else:
+        assert (v[others] == 0).all()
+
+
 @pytest.mark.parametrize('dt', [F32, BF16])
 def test_norm_fp8_many_codes(dt):
     """Over a million values, and groups whose largest value is a multiple of 7:
@@ -418,6 +445,26 @@ def test_gemm_fp8_nan_stays_in_its_row_and_column():
     nan = torch.zeros(70, 192, dtype=torch.bool, device=DEV)
     nan[3], nan[:, 100] = True, True
     assert torch.equal(torch.isnan(out), nan)
+
+
+@pytest.mark.parametrize('m,n', [(70, 192), (900, 16384)])
+def test_gemm_fp8_infinite_scales_stay_in_their_rows(m, n):
+    """As norm_fp8 gives them for a group with an infinity."""
+    g = gen(29)
+    x = randn(g, m, 304)
+    x[3, 140] = math.inf
+    a = torch.empty(m, 304, dtype=E4M3, device=DEV)
+    sa = torch.empty(m, 3, device=DEV)
+    ops.norm_fp8(_lib.NORM_NONE, x, a, sa)
+    inf = torch.zeros(m, 3, dtype=torch.bool, device=DEV)
+    inf[3, 1] = True
+    assert torch.equal(torch.isinf(sa), inf)
+    b, sb = pack.quantize_blocks(randn(g, n, 304))
+    out = torch.empty(m, n, device=DEV)
+    ops.gemm_fp8(a, sa, b, sb, out, epilogue=_lib.EPI_F32_STORE)
+    nan = torch.zeros(m, n, dtype=torch.bool, device=DEV)
+    nan[3] = True
+    assert torch.equal(~torch.isfinite(out), nan)
 
 
 # ------------------------------------------------------------ paged_append
@@ -769,6 +816,49 @@ def test_empty_caches_and_tables(pages, columns, batch):
             ops.paged_append(q, k, k, slots, cache, cache.clone(), q_out=got)
             assert torch.equal(got, q if slot < 0 else torch.zeros_like(q))
             assert ops.device_status(reset=True) == status
+
+
+@pytest.mark.parametrize('dim,page', [(64, 16), (128, 7), (256, 32)])
+@pytest.mark.parametrize('n', [200, 6000])
+def test_paged_attention_values_that_are_not_finite(dim, page, n):
+    """They stay in their head, or in their dimension of it."""
+    g = gen(23)
+    q, kc, vc, table, ln = paged_inputs(g, [40] + [n] * 6, 4, 2, dim, page)
+    ws = workspace(4, 2, dim)
+    good, good_lse = torch.empty_like(q), torch.empty(7, 4, device=DEV)
+    ops.paged_attention(q, kc, vc, table, ln, good, scale=0.125, lse=good_lse,
+                        workspace=ws)
+
+    def row(cache, seq, key):
+        return cache[int(table[seq, key // page]), key % page]
+
+    row(kc, 1, 150)[1, 3] = math.nan
+    row(vc, 2, 17)[0, 5] = math.inf
+    row(vc, 3, 17)[0, 6] = -math.inf
+    row(vc, 3, 33)[0, 7] = math.nan
+    q[4, 2, 0] = math.nan
+    row(kc, 5, 199)[0, 0] = math.inf       # scores of +infinity or -infinity
+    q[5, 0, 0], q[5, 1, 0] = 1.0, -1.0
+    q[6] = q[6].abs() + 0.5                # scores of -infinity, all of them
+    for key in range(n):
+        row(kc, 6, key)[1] = -math.inf
+    out, lse = torch.empty_like(q), torch.empty(7, 4, device=DEV)
+    ops.paged_attention(q, kc, vc, table, ln, out, scale=0.125, lse=lse, workspace=ws)
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[1, 2:] = True
+    bad[2, :2, 5] = True
+    bad[3, :2, 6:8] = True
+    bad[4, 2] = True
+    bad[5, 0] = True
+    assert torch.equal(~torch.isfinite(out), bad)
+    assert torch.equal(torch.isnan(lse), bad.all(-1))
+    assert (out[6, 2:] == 0).all() and (lse[6, 2:] == -math.inf).all()
+    # one key fewer
+    assert torch.isfinite(out[5, 1]).all() and lse[5, 1] != good_lse[5, 1]
+    same = ~bad
+    same[5, 1] = same[6] = False           # other queries
+    assert torch.equal(out[same], good[same])
+    assert torch.equal(lse[same.any(-1)], good_lse[same.any(-1)])
 
 
 def test_paged_attention_offsets_beyond_32_bits():
