@@ -603,6 +603,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       phase ^= 1;
     }
   };
+  // the next tile is here, for all lanes alike: false if the wait ran out
+  auto arrived = [&]() {
+    return __all_sync(0xffffffffu, mbar_wait_spin(&full[slot], phase)) != 0;
+  };
   // queries: B fragments (dims x heads), heads past the group are zero
   uint32_t qf[NT][D / 16][2];
   auto load_q = [&]() {
@@ -636,7 +640,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int e = 0; e < 4; ++e) o[t][j][e] = 0.f;
     }
     for (int i = 0; i < run.n_tiles; ++i) {
-      if (!mbar_wait_spin(&full[slot], phase)) { alive = false; break; }
+      if (!(alive = arrived())) break;
       const int nv = min(SUB, run.len - ((run.k_first + i) * UNIT + warp * SUB));
       // four sums at a time, so that one product does not wait for another
       constexpr int CH = NT == 1 ? 4 : 2;
@@ -706,7 +710,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[t][j][e] *= alpha[t][e & 1];
       }
-      if (!mbar_wait_spin(&full[slot], phase)) { alive = false; break; }
+      if (!(alive = arrived())) break;
       // keys past the last one: their tile rows hold what was there before,
       // which times a weight of zero may still be NaN
       const int kk = 2 * (lane & 3);
@@ -738,8 +742,20 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       advance();
     }
-    // every wait that ran out ends the CTA here, together
-    if (__syncthreads_or(!alive)) return;
+    // every wait that ran out ends the CTA here, together, once the copies that
+    // are still under way into its rings have ended (or had as long again)
+    if (__syncthreads_or(!alive)) {
+      if (!alive) {
+        do {
+          mbar_wait_limit(&full[slot], phase, FVB_WAIT_LIMIT_NS / 8);
+          if (++slot == C::SLOTS) {
+            slot = 0;
+            phase ^= 1;
+          }
+        } while (slot != next);
+      }
+      return;
+    }
 
     // the next run's first tiles arrive while this one is joined; the ring
     // keeps NT slots free, where each warp puts its O
