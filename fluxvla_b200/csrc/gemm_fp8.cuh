@@ -240,7 +240,8 @@ __device__ __forceinline__ bool write_factors(const Dev& p, int t0, int block, i
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       a[i] = p.sa[(long long)min(t0 + i * 8 + r0, p.m - 1) * p.ld_sa + ge];
-    if (!mbar_wait(&fempty[slot], ((bt >> 1) & 1) ^ 1)) return false;
+    // all lanes give up together, or none
+    if (!__all_sync(0xffffffffu, mbar_wait(&fempty[slot], ((bt >> 1) & 1) ^ 1))) return false;
     float* f = fac + slot * (BATCH * 128 * BLOCKS);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
       for (int i0 = 0; i0 < ng && ok; i0 += BATCH) {
         const int batch = MULTI ? bt++ : i0 / BATCH, slot = batch & 1;
-        ok = mbar_wait_spin(&ffull[slot], (batch >> 1) & 1);
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(&ffull[slot], (batch >> 1) & 1));
         const float4 f4 = reinterpret_cast<const float4*>(fac)[slot * 128 + q * 32 + lane];
         __syncwarp();
         if (lane == 0) mbar_arrive(&fempty[slot]);
