@@ -137,6 +137,13 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
   }
 }
 
+// After a wait has run out: waits for the loads that are still under way into a
+// ring, the last of `issued`, as the CTA may not end before them.
+__device__ __forceinline__ void drain(uint64_t* full, int issued, int stages) {
+  for (int i = max(issued - stages, 0); i < issued; ++i)
+    mbar_wait_limit(&full[i % stages], (i / stages) & 1, FVB_WAIT_LIMIT_NS / 8);
+}
+
 // 32 TMEM lanes x 32 columns into registers; tmem_wait makes them valid
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
   asm volatile(
@@ -405,11 +412,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   griddep_wait();
   griddep_launch_dependents();
 
+  bool alive = true;  // no wait of this thread has run out
+  int issued = 0;     // loads of the producer
   if (warp == 0) {
     if (lane == 0) {
       int s = 0;
       uint32_t phase = 1;
-      bool alive = true;
       int w = tile0;
       do {
         const int f = w % p.f_tiles * C::TILE, t = w / p.f_tiles * rows;
@@ -419,6 +427,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           uint8_t* st = smem + s * stage_bytes;
           tma_load_2d(st + a_bytes, &tmB, g * GROUP, f, &full[s]);
           tma_load_2d(st, &tmA, g * GROUP, t, &full[s]);
+          ++issued;
           if (++s == stages) {
             s = 0;
             phase ^= 1;
@@ -440,7 +449,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int b = i % NB;
       bool ready = mbar_wait_spin(&full[s], phase);
       ready = ready && mbar_wait_spin(&tempty[b], ((i / NB) & 1) ^ 1);
-      if (!__all_sync(0xffffffffu, ready)) break;
+      alive = __all_sync(0xffffffffu, ready);
+      if (!alive) break;
       tc_fence_after();
       if (elected) {
         const uint64_t da = smem_desc_sw128(smem_u32(smem + s * stage_bytes));
@@ -462,7 +472,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else if (warp == FACTOR_WARP) {
     int bt = 0;
     int w = tile0;
-    bool alive;
     do {
       alive = write_factors<1>(p, w / p.f_tiles * rows, w % p.f_tiles, g0, g1, fac, ffull, fempty,
                                bt, lane);
@@ -560,9 +569,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             : "memory");
       }
     }
+    alive = ok;
   }
   tc_fence_before();
-  __syncthreads();
+  if (__syncthreads_or(!alive) && threadIdx.x == 0) drain(full, issued, stages);
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
@@ -637,6 +647,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* fempty = ffull + 2;         // [2]
   float* fac = reinterpret_cast<float*>(smem + C::OFF_F);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fempty + 2);
+  // {TMEM address, whether a wait of either CTA has run out, loads issued}
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
@@ -653,6 +664,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&ffull[a], 1);
       mbar_init(&fempty[a], C::SUM_WARPS);
     }
+    tmem_slot[1] = 0;
     fence_barrier_init();
     prefetch_tensormap(&tmA);
     prefetch_tensormap(&tmB);
@@ -677,17 +689,22 @@ __global__ void __launch_bounds__(THREADS, 1)
   // 256 * 208 + 128 * 80 = 63488 <= 384 * 168.  (Sixteen summing warps of 64
   // columns measured 80 us against 71 us on 816 x 32768 x 2048.)
   // Token tiles vary fastest: the pairs at work share weight tiles.
+  auto gave_up = [&]() {
+    for (int c = 0; c < 2; ++c)
+      asm volatile("st.shared::cluster.u32 [%0], 1;" ::"r"(mapa(smem_u32(tmem_slot + 1), c))
+                   : "memory");
+  };
   if (warp < FIRST_SUM_WARP) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    bool alive = true;
     if (warp == 0 && lane == 0) {
-      int it = 0;
-      bool alive = true;
+      int issued = 0;
       for (int w = pair; w < n_tiles && alive; w += n_pairs) {
         const int trow = (w % p.t_tiles) * C::TILE + (int)rank * 128;
         const int wrow = (w / p.t_tiles) * C::TILE + (int)rank * 128;
-        for (int g = 0; g < p.groups; ++g, ++it) {
-          const int s = it % C::STAGES;
-          if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1)) { alive = false; break; }
+        for (int g = 0; g < p.groups; ++g, ++issued) {
+          const int s = issued % C::STAGES;
+          if (!mbar_wait(&empty[s], ((issued / C::STAGES) & 1) ^ 1)) { alive = false; break; }
           const uint32_t fb = mapa(smem_u32(&full[s]), 0);
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * C::STAGE);
           uint8_t* sa = smem + s * C::STAGE;
@@ -695,6 +712,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           tma_load_2d_pair(sa + C::HALF, &tmB, g * GROUP, wrow, fb);
         }
       }
+      tmem_slot[2] = issued;
     } else if (warp == 1 && rank == 0) {
       constexpr uint32_t IDESC = idesc_e4m3_f32(256, C::TILE);
       const bool elected = elect_one();
@@ -706,7 +724,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int b = it & 1;
         bool ready = mbar_wait_spin(&full[s], phase);
         ready = ready && mbar_wait_cluster(&tempty[b], ((it >> 1) & 1) ^ 1);
-        if (!__all_sync(0xffffffffu, ready)) break;
+        alive = __all_sync(0xffffffffu, ready);
+        if (!alive) break;
         tc_fence_after();
         if (elected) {
           const uint64_t da = smem_desc_sw128(smem_u32(smem + s * C::STAGE));
@@ -725,11 +744,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     } else if (warp == FACTOR_WARP) {
       int bt = 0;
-      bool alive = true;
       for (int w = pair; w < n_tiles && alive; w += n_pairs)
         alive = write_factors<2>(p, (w % p.t_tiles) * C::TILE + (int)rank * 128,
                                  (w / p.t_tiles) * 2, 0, p.groups, fac, ffull, fempty, bt, lane);
     }
+    if (!alive) gave_up();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int q = warp & 3, part = (warp - FIRST_SUM_WARP) >> 2;
@@ -777,7 +796,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           scale_add<32>(acc + 32 * j, r[j & 1], f);
         }
       }
-      if (!ok) break;
+      if (!ok) {
+        gave_up();
+        break;
+      }
       // A lane holds one token's features: 64 bytes of output a row at a time
       // go through shared memory (16-byte pieces swizzled by the row), so that
       // each store instruction writes 64 bytes of 8 rows.
@@ -851,6 +873,19 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncwarp();
   cluster_arrive();  // every MMA, commit and remote arrival is done
   cluster_wait();
+  if (tmem_slot[1]) {
+    // the loads of both CTAs arrive at the leader's barriers; those that the
+    // leader does not expect have the time of one wait
+    if (threadIdx.x == 0) {
+      if (rank == 0)
+        drain(full, tmem_slot[2], C::STAGES);
+      else
+        mbar_wait_limit(&full[0], 0, FVB_WAIT_LIMIT_NS / 8);
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  }
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
