@@ -30,7 +30,8 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
 }
 
 __device__ __forceinline__ void record_device_error(int code) {
-  atomicCAS(&g_fvb_device_status, 0, code);
+  // a wait that ran out (4) outranks a bad argument (1), whichever came first
+  atomicMax(&g_fvb_device_status, code);
 }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

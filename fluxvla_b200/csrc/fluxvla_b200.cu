@@ -273,7 +273,7 @@ int fvb_get_device_status(int* status, int reset) {
   // the serving operators' kernels have a status word of their own
   int other = FVB_OK;
   if (int r = fvb_serving_device_status(&other, reset)) return r;
-  if (*status == FVB_OK) *status = other;
+  if (other > *status) *status = other;
   return FVB_OK;
 }
 
