@@ -10,13 +10,13 @@
 // factor sa * sb of a group is one register for all its columns.  (With the
 // features there, few tokens would not waste rows of the tensor core, but the
 // factor would vary along the columns and come from shared memory for every
-// product: 13.7 us against 12.5 us on 64 x 2048 x 16384.)
+// product: 13.7 us against 12.6 us on 64 x 2048 x 16384.)
 //
 //   warp 0      TMA producer: ring of (tokens, weights) tiles of 128-byte rows
 //   warp 1      tcgen05.mma issuer; the cluster kernel has a second one, warp 3,
 //               for every other group: one takes longer over a group's waits,
 //               MMAs and commits than a 128 x 128 product does (13.5 us
-//               against 12.5 us on 64 x 2048 x 16384)
+//               against 12.6 us on 64 x 2048 x 16384)
 //   warp 2      factors, four groups at a time, two batches ahead
 //   warps 4..11 read TMEM (warp w: lanes 32*(w%4)..+31, half of the columns),
 //               multiply by the factors, accumulate
@@ -629,8 +629,8 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster) {
                : "memory");
 }
 // VEC: rows of out start and end on 16 bytes.  (A kernel of its own for the
-// others: with both in one the sums spill, 71 us become 86 on 816 x 32768 x
-// 2048.)
+// others, 87 us against 74 us on 816 x 32764 x 2048: with both in one the sums
+// spill, and the aligned one took 86 us too.)
 template <int EPI, bool VEC>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_fp8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,

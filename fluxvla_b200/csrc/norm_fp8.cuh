@@ -228,7 +228,9 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
 }
 
 // y / s rounded to odd (toward zero, and the last bit set where that was not
-// exact), which rounds to e4m3 as y / s itself does; y0, y1 >= 0 that f32
+// exact), which rounds to e4m3 as y / s itself does (Boldo and Melquiond,
+// Emulation of FMA and correctly rounded sums: proved algorithms using rounding
+// to odd, IEEE Transactions on Computers 57, 2008); y0, y1 >= 0 that f32
 // holds, r = 1 / s within an ulp.  t is the quotient within its last bit, so
 // that the remainder y - t s, rounded once, has the sign of the error.
 __device__ __forceinline__ void divide_odd(float y0, float y1, float s, float r, float& t0,

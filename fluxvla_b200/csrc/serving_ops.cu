@@ -325,8 +325,11 @@ int fvb_gemm_fp8(const fvb_gemm_fp8_args* a, void* stream) {
   // The shape with the least time by a count of clocks, fitted to measured
   // products: a group costs the cluster kernel 600 clocks, a call 3000, a tile
   // 1500 more (3000 with an exchange), the pair kernel 970 and 3500 for a tile
-  // of twice the height and width.  816 x 32768 x 2048: pair 70 us, clusters 109 us;
-  // 816 x 2560 x 2048: the other way round, 40 pair tiles leave SMs idle.
+  // of twice the height and width.  816 x 32768 x 2048 GEGLU at 1965 MHz: pair
+  // 74 us, clusters 109 us; 816 x 2560 x 2048: the other way round, 40 pair tiles
+  // leave SMs idle.  The count ranks shapes; where rows are no multiple of 128
+  // bytes and a tile is 128 rows high it is far too low (768 x 1152 x 4304: 8.2 us
+  // counted, 15 us taken).
   if (int rr = ensure_smem(cluster_kernel<false>(FVB_EPI_BF16), fvb::g8::ClusterCfg::MAX_SMEM,
                            "fvb_gemm_fp8"))
     return rr;

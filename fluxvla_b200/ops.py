@@ -219,7 +219,8 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
     (fvb_gemm_fp8): a [M, K] with a_scale [M, ceil(K / 128)] as norm_fp8 gives
     them, b [N, K] with b_scale [ceil(N / 128), ceil(K / 128)] as
     pack.quantize_blocks lays them out.  EPI_BF16, EPI_F32_STORE, or EPI_GEGLU
-    (rows of b packed by pack.pack_geglu, out [M, N / 2])."""
+    (rows of b packed by pack.pack_geglu, out [M, N / 2]).  Rows of a and b
+    start on 16 bytes (a K that is no multiple of 16 needs wider buffers)."""
     _C().gemm_fp8(a, a_scale, b, b_scale, out, epilogue)
 
 

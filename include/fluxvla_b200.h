@@ -410,7 +410,7 @@ typedef struct fvb_paged_append_args {
  * outside the table too.  A slot past the cache, or a cached token's position
  * outside the table, writes nothing and sets FVB_ERR_INVALID_ARG in the device
  * status word.  Slots of one call are distinct: of two tokens with the same
- * slot it is not defined which one's values stay.                           */
+ * slot it is not defined whose values stay, value by value.                  */
 int fvb_paged_append(const fvb_paged_append_args* args, void* stream);
 
 typedef struct fvb_paged_attn_args {
