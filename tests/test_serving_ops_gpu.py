@@ -1121,3 +1121,47 @@ def test_layers_back_to_back_equal_layers_call_by_call(tokens):
         graph.replay()
         assert all(torch.equal(x, y) for x, y in zip(a, graphed.state()))
     assert ops.device_status() == 0
+
+
+def test_operators_on_streams_of_their_own():
+    """Products of both kernels, norms and attention side by side, in an order
+    that changes, give what each gives alone."""
+    g = gen(30)
+    jobs = []
+    for m, n, k, epi in ((816, 8192, 2048, 'geglu'), (64, 2048, 4096, 'f32'),
+                         (1, 2560, 2048, 'bf16'), (768, 1152, 4304, 'bf16'),
+                         (2000, 4096, 1024, 'bf16')):
+        args = gemm_inputs(g, m, n, k)
+        out = torch.empty(m, n // 2 if epi == 'geglu' else n, device=DEV,
+                          dtype=F32 if epi == 'f32' else BF16)
+        jobs.append((lambda args=args, out=out, epi=epi: ops.gemm_fp8(
+            *args, out, epilogue=EPIS[epi]), [out]))
+    for lens, heads, kv, dim, page in (([3000] * 20, 8, 1, 128, 16),
+                                       ([9000], 8, 2, 64, 7),
+                                       (list(range(100, 164)), 16, 1, 256, 32)):
+        args = paged_inputs(g, lens, heads, kv, dim, page)
+        out, lse = torch.empty_like(args[0]), torch.empty(len(lens), heads, device=DEV)
+        ws = workspace(heads, kv, dim)
+        jobs.append((lambda args=args, out=out, lse=lse, ws=ws: ops.paged_attention(
+            *args, out, scale=0.1, lse=lse, workspace=ws), [out, lse]))
+    x = randn(g, 2000, 2048)
+    q = torch.empty(2000, 2048, dtype=E4M3, device=DEV)
+    s = torch.empty(2000, 16, device=DEV)
+    jobs.append((lambda: ops.norm_fp8(_lib.NORM_RMS, x, q, s), [q.view(torch.uint8), s]))
+    want = []
+    for call, outs in jobs:
+        call()
+        want.append([t.clone() for t in outs])
+        for t in outs:
+            t.fill_(3)
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for i in range(60):
+        for j in range(len(jobs)):
+            j = (j * 4 + i) % len(jobs)          # 9 jobs: 4 is prime to them
+            with torch.cuda.stream(streams[j]):
+                jobs[j][0]()
+    torch.cuda.synchronize()
+    for (_, outs), ref in zip(jobs, want):
+        assert all(torch.equal(a, b) for a, b in zip(outs, ref))
+    assert ops.device_status() == 0
